@@ -301,6 +301,71 @@ int b200_step_metadata(const int* seq_info, const int* block_tables, int bt_stri
                        int* context_lens, b200_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Pages of the KV cache
+ * ------------------------------------------------------------------------
+ * No counterpart in the reference, whose BlockManager (src/engine/
+ * block_manager.py:47) keeps its tables on the host and never copies a page.
+ *  - cache: n0 x n1 planes (K or V of one layer), each of num_pages pages of
+ *    `page` slots of slot_bytes (the bytes of one token's K or V in one
+ *    layer).  Byte strides: s0 / s1 between planes, page_stride between pages;
+ *    slots are contiguous in a page.  Everything a multiple of 16 bytes.
+ *  - block_tables: int32 [rows][width], bt_stride entries apart, the pages of
+ *    each row in order, -1 behind them; seq_lens: int32 [rows], a row of n
+ *    tokens holds ceil(n / page) pages; refs: int32 [num_pages], the rows that
+ *    hold each page, 0 for a free one.
+ *  - Index arrays are int32 on the device; an entry of -1 is skipped (padding),
+ *    any other one outside its range is skipped and flags
+ *    B200_DEVERR_BAD_INDEX.
+ *  - Free pages are taken lowest first, in the order of the requests: results
+ *    do not depend on timing.  Calls that change the same tables must not
+ *    overlap on the GPU. */
+
+/* The first num_tokens[i] slots (NULL: the whole page) of page src[i] into
+ * page dst[i] in every plane, i < n.  One source may have several
+ * destinations; a page that is a destination twice, or a source and a
+ * destination of different copies, holds a mixture afterwards (and nothing
+ * outside it changes). */
+int b200_copy_pages(void* cache, long long s0, long long s1, long long page_stride, int n0, int n1,
+                    int num_pages, int page, long long slot_bytes, const int* src, const int* dst,
+                    const int* num_tokens, int n, b200_stream_t stream);
+
+/* Row row_ids[i] grows to new_lens[i] tokens: it gets the pages it lacks, with
+ * one reference each.  done[i] = 1, or 0 with the row left as it was: when it
+ * would shrink or pass `width` pages, when the row is listed before, or when
+ * the pages that rows 0..i of the list need are more than there are free
+ * pages.  n <= 1024 (B200_ERR_UNSUPPORTED otherwise). */
+int b200_take_pages(int* block_tables, long long bt_stride, int rows, int width, int* seq_lens, int* refs,
+                    int num_pages, int page, const int* row_ids, const int* new_lens, int n, int* done,
+                    b200_stream_t stream);
+
+/* Rows row_ids[i] give their pages back: one reference less for each, the row
+ * filled with -1, its length 0.  A row may be listed twice. */
+int b200_free_pages(int* block_tables, long long bt_stride, int rows, int width, int* seq_lens, int* refs,
+                    int num_pages, const int* row_ids, int n, b200_stream_t stream);
+
+/* Row children[i] becomes a fork of row parents[i]: it shares the parent's
+ * full pages (one reference more for each) and gets a copy, on the lowest free
+ * page, of the used slots of a last page that is not full, so that both rows
+ * can go on.  All parents are read as they are before the call.  done[i] = 1,
+ * or 0 with nothing changed: when the child's length is not 0 (free it
+ * first), when the child is listed before, or when no free page is left for
+ * it.  n <= 1024.  plan: int32 [n][4] of scratch, 16-byte aligned. */
+int b200_fork_pages(void* cache, long long s0, long long s1, long long page_stride, int n0, int n1,
+                    int num_pages, int page, long long slot_bytes, int* block_tables, long long bt_stride,
+                    int rows, int width, int* seq_lens, int* refs, const int* parents, const int* children,
+                    int n, int* plan, int* done, b200_stream_t stream);
+
+/* With N live pages (refs != 0), moves them into pages [0, N): the k-th live
+ * page at N or behind takes the place of the k-th free page before N.  Its
+ * contents are copied in every plane, refs and the tables follow.
+ * place[p] (int32 [num_pages]) is where page p's contents are afterwards, -1
+ * for a free page; moves: int32 [2 + num_pages] of scratch, the number of moved
+ * pages in moves[0]. */
+int b200_compact_pages(void* cache, long long s0, long long s1, long long page_stride, int n0, int n1,
+                       int num_pages, int page, long long slot_bytes, int* block_tables, long long bt_stride,
+                       int rows, int width, int* refs, int* place, int* moves, b200_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Vocabulary
  * ------------------------------------------------------------------------ */
 

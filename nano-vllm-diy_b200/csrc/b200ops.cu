@@ -22,6 +22,7 @@
 #include "elementwise.cuh"
 #include "exchange.cuh"
 #include "metadata.cuh"
+#include "pages.cuh"
 #include "prefill_tc.cuh"
 #include "gemm.cuh"
 #include "gemm_pair.cuh"
@@ -1527,4 +1528,141 @@ extern "C" int b200_paged_decode_attention_static(
   if (int r = ensure_smem(ds, 2u, decode_attn_kernel, smem)) return r;
   if (int r = launch_decode(ds, tmK, tmV, tmQ, a, smem, st)) return r;
   return check_launch("decode_attn_kernel");
+}
+
+// ===========================================================================
+// Pages of the KV cache (pages.cuh)
+// ===========================================================================
+namespace {
+
+// Fills `c` from byte strides; every plane, page and slot is a whole number of
+// 16-byte vectors, so all copies are vector copies.
+int page_cache(const char* what, void* cache, long long s0, long long s1, long long page_stride, int n0, int n1,
+               int num_pages, int page, long long slot_bytes, PageCache* c) {
+  if (!cache || !aligned16(cache) || n0 <= 0 || n1 <= 0 || num_pages <= 0 || page <= 0 || slot_bytes <= 0)
+    return fail(B200_ERR_INVALID, "%s: cache missing, misaligned or empty", what);
+  if (slot_bytes % 16 || s0 % 16 || s1 % 16 || page_stride % 16)
+    return fail(B200_ERR_UNSUPPORTED, "%s: slots and strides must be multiples of 16 bytes", what);
+  if ((long long)page * slot_bytes / 16 > (1LL << 30) || (long long)n0 * n1 > (1 << 20))
+    return fail(B200_ERR_UNSUPPORTED, "%s: pages of %d slots of %lld bytes in %d x %d planes", what, page, slot_bytes,
+                n0, n1);
+  if (s0 < 0 || s1 < 0 || page_stride < (num_pages > 1 ? page * slot_bytes : 0) || (n0 > 1 && s0 == 0) ||
+      (n1 > 1 && s1 == 0))
+    return fail(B200_ERR_INVALID, "%s: planes or pages of the cache overlap", what);
+  c->base = static_cast<uint4*>(cache);
+  c->s0 = s0 / 16;
+  c->s1 = s1 / 16;
+  c->page_stride = page_stride / 16;
+  c->n1 = n1;
+  c->planes = n0 * n1;
+  c->slot_vecs = (int)(slot_bytes / 16);
+  c->page_vecs = (int)(page * slot_bytes / 16);
+  return B200_OK;
+}
+
+int page_tables(const char* what, int* block_tables, long long bt_stride, int rows, int width, int* seq_lens,
+                int* refs, int num_pages, int page, PageTables* t) {
+  if (!block_tables || !refs || rows <= 0 || width <= 0 || num_pages <= 0 || page <= 0 || bt_stride < width)
+    return fail(B200_ERR_INVALID, "%s: rows=%d width=%d (stride %lld) pages=%d of %d", what, rows, width, bt_stride,
+                num_pages, page);
+  if (width > (1 << 20) || (long long)width * page > 0x7fffffffLL || num_pages > (1 << 30))
+    return fail(B200_ERR_UNSUPPORTED, "%s: lengths of %d pages of %d tokens pass 31 bits", what, width, page);
+  DeviceState* ds;
+  if (int r = device_state(&ds)) return r;
+  *t = PageTables{block_tables, bt_stride, rows, width, seq_lens, refs, num_pages, page, ds->err};
+  return B200_OK;
+}
+
+// One resident wave of content CTAs (4 of 256 threads on each SM keep 128 KB
+// of loads in flight), or one CTA per unit when there are fewer.
+int page_grid(long long units) {
+  DeviceState* ds;
+  if (device_state(&ds)) return 1;
+  return (int)std::max<long long>(1, std::min<long long>(units, (long long)ds->num_sms * 4));
+}
+
+}  // namespace
+
+extern "C" int b200_copy_pages(void* cache, long long s0, long long s1, long long page_stride, int n0, int n1,
+                               int num_pages, int page, long long slot_bytes, const int* src, const int* dst,
+                               const int* num_tokens, int n, b200_stream_t stream) {
+  if (n <= 0) return B200_OK;
+  PageCache c{};
+  if (int r = page_cache("copy_pages", cache, s0, s1, page_stride, n0, n1, num_pages, page, slot_bytes, &c)) return r;
+  if (!src || !dst) return fail(B200_ERR_INVALID, "copy_pages: null pointer");
+  DeviceState* ds;
+  if (int r = device_state(&ds)) return r;
+  const long long units = (long long)n * c.planes * ((c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs);
+  launch_ex(copy_pages_kernel, dim3(page_grid(units)), dim3(kPgThreads), 0, reinterpret_cast<cudaStream_t>(stream),
+            nullptr, 0, c, src, dst, num_tokens, n, num_pages, page, ds->err);
+  return check_launch("copy_pages_kernel");
+}
+
+extern "C" int b200_take_pages(int* block_tables, long long bt_stride, int rows, int width, int* seq_lens, int* refs,
+                               int num_pages, int page, const int* row_ids, const int* new_lens, int n, int* done,
+                               b200_stream_t stream) {
+  if (n <= 0) return B200_OK;
+  if (n > kPgMax) return fail(B200_ERR_UNSUPPORTED, "take_pages: %d rows in one call (at most %d)", n, kPgMax);
+  if (!seq_lens || !row_ids || !new_lens || !done) return fail(B200_ERR_INVALID, "take_pages: null pointer");
+  PageTables t{};
+  if (int r = page_tables("take_pages", block_tables, bt_stride, rows, width, seq_lens, refs, num_pages, page, &t))
+    return r;
+  launch_ex(take_pages_kernel, dim3(1), dim3(kPgMax), 0, reinterpret_cast<cudaStream_t>(stream), nullptr, 0, t,
+            row_ids, new_lens, n, done);
+  return check_launch("take_pages_kernel");
+}
+
+extern "C" int b200_free_pages(int* block_tables, long long bt_stride, int rows, int width, int* seq_lens, int* refs,
+                               int num_pages, const int* row_ids, int n, b200_stream_t stream) {
+  if (n <= 0) return B200_OK;
+  if (!seq_lens || !row_ids) return fail(B200_ERR_INVALID, "free_pages: null pointer");
+  PageTables t{};
+  if (int r = page_tables("free_pages", block_tables, bt_stride, rows, width, seq_lens, refs, num_pages, 1, &t))
+    return r;
+  launch_ex(free_pages_kernel, dim3(n), dim3(kPgThreads), 0, reinterpret_cast<cudaStream_t>(stream), nullptr, 0, t,
+            row_ids);
+  return check_launch("free_pages_kernel");
+}
+
+extern "C" int b200_fork_pages(void* cache, long long s0, long long s1, long long page_stride, int n0, int n1,
+                               int num_pages, int page, long long slot_bytes, int* block_tables, long long bt_stride,
+                               int rows, int width, int* seq_lens, int* refs, const int* parents, const int* children,
+                               int n, int* plan, int* done, b200_stream_t stream) {
+  if (n <= 0) return B200_OK;
+  if (n > kPgMax) return fail(B200_ERR_UNSUPPORTED, "fork_pages: %d forks in one call (at most %d)", n, kPgMax);
+  if (!seq_lens || !parents || !children || !done || !plan || !aligned16(plan))
+    return fail(B200_ERR_INVALID, "fork_pages: null pointer or plan not 16-byte aligned");
+  PageCache c{};
+  if (int r = page_cache("fork_pages", cache, s0, s1, page_stride, n0, n1, num_pages, page, slot_bytes, &c)) return r;
+  PageTables t{};
+  if (int r = page_tables("fork_pages", block_tables, bt_stride, rows, width, seq_lens, refs, num_pages, page, &t))
+    return r;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  launch_ex(fork_plan_kernel, dim3(1), dim3(kPgMax), 0, st, nullptr, 0, t, parents, children, n, plan, done);
+  if (int r = check_launch("fork_plan_kernel")) return r;
+  const long long units = n + (long long)n * c.planes * ((c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs);
+  launch_ex(fork_apply_kernel, dim3(page_grid(units)), dim3(kPgThreads), 0, st, nullptr, 0, t, c, parents, children,
+            n, static_cast<const int*>(plan));
+  return check_launch("fork_apply_kernel");
+}
+
+extern "C" int b200_compact_pages(void* cache, long long s0, long long s1, long long page_stride, int n0, int n1,
+                                  int num_pages, int page, long long slot_bytes, int* block_tables,
+                                  long long bt_stride, int rows, int width, int* refs, int* place, int* moves,
+                                  b200_stream_t stream) {
+  if (!place || !moves) return fail(B200_ERR_INVALID, "compact_pages: null pointer");
+  PageCache c{};
+  if (int r = page_cache("compact_pages", cache, s0, s1, page_stride, n0, n1, num_pages, page, slot_bytes, &c))
+    return r;
+  PageTables t{};
+  if (int r = page_tables("compact_pages", block_tables, bt_stride, rows, width, nullptr, refs, num_pages, page, &t))
+    return r;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  launch_ex(compact_plan_kernel, dim3(1), dim3(kPgMax), 0, st, nullptr, 0, t, place, moves);
+  if (int r = check_launch("compact_plan_kernel")) return r;
+  const long long pieces = (c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs;
+  const long long units = ((long long)rows * width + kPgThreads - 1) / kPgThreads + num_pages / 2 * c.planes * pieces;
+  launch_ex(compact_apply_kernel, dim3(page_grid(units)), dim3(kPgThreads), 0, st, nullptr, 0, t, c,
+            static_cast<const int*>(place), static_cast<const int*>(moves));
+  return check_launch("compact_apply_kernel");
 }

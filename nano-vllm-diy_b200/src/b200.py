@@ -13,6 +13,7 @@ and are reused by every call.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -71,6 +72,17 @@ _SIGNATURES = {
                                     ctypes.c_ulonglong, ctypes.c_ulonglong, _c_void_p, _c_void_p], _i),
     "b200_select_tokens_exchange": ([_c_void_p, _i, _i, _i, _c_void_p, _c_void_p, _c_void_p, _ll,
                                      _c_void_p, _c_void_p], _i),
+    "b200_copy_pages": ([_c_void_p, _ll, _ll, _ll, _i, _i, _i, _i, _ll, _c_void_p, _c_void_p,
+                         _c_void_p, _i, _c_void_p], _i),
+    "b200_take_pages": ([_c_void_p, _ll, _i, _i, _c_void_p, _c_void_p, _i, _i, _c_void_p, _c_void_p,
+                         _i, _c_void_p, _c_void_p], _i),
+    "b200_free_pages": ([_c_void_p, _ll, _i, _i, _c_void_p, _c_void_p, _i, _c_void_p, _i,
+                         _c_void_p], _i),
+    "b200_fork_pages": ([_c_void_p, _ll, _ll, _ll, _i, _i, _i, _i, _ll, _c_void_p, _ll, _i, _i,
+                         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i, _c_void_p, _c_void_p,
+                         _c_void_p], _i),
+    "b200_compact_pages": ([_c_void_p, _ll, _ll, _ll, _i, _i, _i, _i, _ll, _c_void_p, _ll, _i, _i,
+                            _c_void_p, _c_void_p, _c_void_p, _c_void_p], _i),
     "b200_attention_workspace_bytes": ([_i, _i, _i, ctypes.POINTER(_sz)], _i),
     "b200_paged_decode_attention_static": ([_c_void_p, _ll, _i, _c_void_p, _c_void_p, _ll,
                                             _c_void_p, _i, _i, _c_void_p, _c_void_p, _i, _i,
@@ -555,6 +567,139 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | N
         float(softmax_scale), _p(out), out.stride(0), _p(ws), nbytes, _stream()),
         "b200_paged_attention")
     return out
+
+
+# ---------------------------------------------------------------------------
+# pages of the KV cache
+# ---------------------------------------------------------------------------
+_SAME = contextlib.nullcontext()
+
+
+def _device_of(*ts: torch.Tensor | None):
+    """A context in which the current device (and so the current stream) is
+    that of the tensors, which must all be on one."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("b200 kernels need CUDA tensors (there is no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return _SAME if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _index(name: str, t: torch.Tensor, n: int | None = None) -> int:
+    """Entries of an int32 vector the kernels index as t[i]."""
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32")
+    if t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1) or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} must be a contiguous vector" + (f" of {n}" if n is not None else ""))
+    return t.shape[0]
+
+
+def _cache_args(kv_cache: torch.Tensor):
+    """C arguments of a cache [pages, page, Hkv, D] with up to two leading plane
+    dimensions (the runner's [2, layers, pages, page, Hkv, D]) and contiguous pages."""
+    d = kv_cache.dim()
+    if d < 4 or d > 6:
+        raise ValueError("kv_cache must be [pages, page, heads, dim], with up to two leading dimensions")
+    shape, stride, size = kv_cache.shape, kv_cache.stride(), kv_cache.element_size()
+    pages, page, heads, dim = shape[-4:]
+    if stride[-1] != 1 or stride[-2] != dim or stride[-3] != heads * dim:
+        raise ValueError("kv_cache: the slots of a page must be contiguous")
+    n0, s0 = (shape[0], stride[0]) if d == 6 else (1, 0)
+    n1, s1 = (shape[d - 5], stride[d - 5]) if d >= 5 else (1, 0)
+    return (kv_cache.data_ptr(), s0 * size, s1 * size, stride[-4] * size, n0, n1, pages, page, heads * dim * size)
+
+
+def _table_args(block_tables: torch.Tensor, seq_lens: torch.Tensor | None, refs: torch.Tensor):
+    if block_tables.dtype != torch.int32:
+        raise TypeError("block_tables must be int32")
+    if block_tables.dim() != 2 or block_tables.stride(1) != 1:
+        raise ValueError("block_tables must be [rows, width] with contiguous rows")
+    rows, width = block_tables.shape
+    if seq_lens is not None:
+        _index("seq_lens", seq_lens, rows)
+    _index("refs", refs)
+    return block_tables.data_ptr(), block_tables.stride(0) if rows > 1 else width, rows, width
+
+
+def copy_pages(kv_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+               num_tokens: torch.Tensor | None = None) -> None:
+    """kv_cache[..., dst[i], :num_tokens[i]] = kv_cache[..., src[i], :num_tokens[i]] in every plane
+    (whole pages without num_tokens).  int32 indices on the device, -1 skips; no page may be the
+    destination of two copies, or the source of one and the destination of another."""
+    with _device_of(kv_cache, src, dst, num_tokens):
+        n = _index("src", src)
+        _index("dst", dst, n)
+        if num_tokens is not None:
+            _index("num_tokens", num_tokens, n)
+        _check(load_library().b200_copy_pages(*_cache_args(kv_cache), _p(src), _p(dst), _p(num_tokens), n,
+                                              _stream()), "b200_copy_pages")
+
+
+def take_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor,
+               new_lens: torch.Tensor, page: int) -> torch.Tensor:
+    """The rows grow to new_lens tokens and get the pages they lack, lowest free ones first in the
+    order of the list.  Returns int32 done [n]: 0 where a row stays as it was (it would shrink or
+    outgrow its table, is listed before, or the list up to it needs more pages than are free)."""
+    with _device_of(block_tables, seq_lens, refs, rows, new_lens):
+        n = _index("rows", rows)
+        _index("new_lens", new_lens, n)
+        tables = _table_args(block_tables, seq_lens, refs)
+        done = torch.empty_like(rows)
+        _check(load_library().b200_take_pages(*tables, _p(seq_lens), _p(refs), refs.shape[0], int(page), _p(rows),
+                                              _p(new_lens), n, _p(done), _stream()), "b200_take_pages")
+    return done
+
+
+def free_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor) -> None:
+    """The rows give their pages back (one reference less for each) and are empty afterwards."""
+    with _device_of(block_tables, seq_lens, refs, rows):
+        n = _index("rows", rows)
+        tables = _table_args(block_tables, seq_lens, refs)
+        _check(load_library().b200_free_pages(*tables, _p(seq_lens), _p(refs), refs.shape[0], _p(rows), n,
+                                              _stream()), "b200_free_pages")
+
+
+def fork_pages(kv_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor,
+               parents: torch.Tensor, children: torch.Tensor) -> torch.Tensor:
+    """Row children[i] (empty) becomes a fork of row parents[i]: the parent's full pages shared, the
+    used part of a last page that is not full copied to the lowest free page.  Returns int32 done
+    [n]: 0 where nothing changed (the child is not empty or listed before, or no page is left)."""
+    with _device_of(kv_cache, block_tables, seq_lens, refs, parents, children):
+        n = _index("parents", parents)
+        _index("children", children, n)
+        cache = _cache_args(kv_cache)
+        tables = _table_args(block_tables, seq_lens, refs)
+        if refs.shape[0] != cache[6]:
+            raise ValueError(f"refs of {refs.shape[0]} pages for a cache of {cache[6]}")
+        # plan and result in one allocation: [n][4] words of scratch, then done
+        out = torch.empty(5 * n, dtype=torch.int32, device=parents.device)
+        done = out[4 * n:]
+        _check(load_library().b200_fork_pages(*cache, *tables, _p(seq_lens), _p(refs), _p(parents), _p(children), n,
+                                              _p(out), _p(done), _stream()), "b200_fork_pages")
+    return done
+
+
+def compact_pages(kv_cache: torch.Tensor, block_tables: torch.Tensor, refs: torch.Tensor) -> torch.Tensor:
+    """Moves the N live pages (refs != 0) into pages [0, N): the k-th live page behind them into the
+    k-th free one among them; tables and refs follow.  Returns int32 place [pages]: where each
+    page's contents are now, -1 for a free page."""
+    with _device_of(kv_cache, block_tables, refs):
+        cache = _cache_args(kv_cache)
+        tables = _table_args(block_tables, None, refs)
+        pages = cache[6]
+        if refs.shape[0] != pages:
+            raise ValueError(f"refs of {refs.shape[0]} pages for a cache of {pages}")
+        place = torch.empty_like(refs)
+        moves = torch.empty(2 + pages, dtype=torch.int32, device=refs.device)
+        _check(load_library().b200_compact_pages(*cache, *tables, _p(refs), _p(place), _p(moves), _stream()),
+               "b200_compact_pages")
+    return place
 
 
 # ---------------------------------------------------------------------------

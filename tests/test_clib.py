@@ -134,3 +134,61 @@ def test_every_python_op_refuses_cpu_tensors():
     for call in calls:
         with pytest.raises(RuntimeError, match="CUDA tensors"):
             call()
+
+
+def test_page_operators_refuse_bad_arguments_before_any_launch():
+    """Shapes, alignment and overlap of the cache are checked on the host."""
+    from src import b200
+    lib = b200.load_library()
+    p = ctypes.c_void_p(16)
+    slot, page = 256, 16
+    cache = [p, 1 << 20, 1 << 16, page * slot, 2, 3, 8, page, slot]
+
+    def copy(c, n=2, src=p):
+        return lib.b200_copy_pages(*c, src, p, None, n, None)
+
+    for at, value, rc in [(0, None, -1), (0, ctypes.c_void_p(8), -1), (4, 0, -1), (6, 0, -1), (7, -1, -1),
+                          (8, 24, -2), (1, 8, -2), (3, 40, -2), (3, 0, -1), (3, page * slot - 16, -1), (1, 0, -1),
+                          (2, -16, -1), (7, 1 << 30, -2)]:
+        c = list(cache)
+        c[at] = value
+        assert copy(c) == rc, (at, value)
+    assert copy(cache, src=None) == -1
+    assert copy([None] * 1 + cache[1:], n=0) == 0  # nothing to do
+    tables = [p, 8, 4, 8]
+    assert lib.b200_take_pages(*tables, p, p, 8, 16, p, p, 1025, p, None) == -2
+    assert lib.b200_take_pages(*tables, p, p, 8, 16, p, None, 4, p, None) == -1
+    assert lib.b200_take_pages(p, 7, 4, 8, p, p, 8, 16, p, p, 4, p, None) == -1  # rows overlap
+    assert lib.b200_take_pages(p, 1 << 20, 4, 1 << 20, p, p, 8, 4096, p, p, 4, p, None) == -2  # 2^32 tokens
+    assert lib.b200_free_pages(*tables, None, p, 8, p, 4, None) == -1
+    assert lib.b200_fork_pages(*cache, *tables, p, p, p, p, 1025, p, p, None) == -2
+    assert lib.b200_fork_pages(*cache, *tables, p, p, p, p, 4, ctypes.c_void_p(8), p, None) == -1
+    assert lib.b200_compact_pages(*cache, *tables, p, None, p, None) == -1
+
+
+def test_page_operators_refuse_cpu_tensors_types_and_layouts():
+    import pytest
+    import torch
+    from src import b200
+    kv = torch.zeros(2, 1, 4, 16, 1, 8, dtype=torch.bfloat16)
+    table = torch.full((3, 2), -1, dtype=torch.int32)
+    lens, refs, idx = (torch.zeros(n, dtype=torch.int32) for n in (3, 4, 2))
+    for call in (lambda: b200.copy_pages(kv, idx, idx), lambda: b200.take_pages(table, lens, refs, idx, idx, 16),
+                 lambda: b200.free_pages(table, lens, refs, idx),
+                 lambda: b200.fork_pages(kv, table, lens, refs, idx, idx),
+                 lambda: b200.compact_pages(kv, table, refs)):
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            call()
+    with pytest.raises(TypeError, match="int32"):
+        b200._index("rows", idx.long())
+    with pytest.raises(ValueError, match="vector of 3"):
+        b200._index("rows", idx, 3)
+    with pytest.raises(ValueError, match="contiguous"):
+        b200._index("rows", torch.zeros(4, dtype=torch.int32)[::2])
+    with pytest.raises(ValueError, match="contiguous"):
+        b200._cache_args(kv.transpose(-2, -3))
+    with pytest.raises(ValueError, match="contiguous rows"):
+        b200._table_args(table.t(), lens, refs)
+    # planes and their strides, in bytes
+    assert b200._cache_args(kv)[1:] == (1024, 1024, 256, 2, 1, 4, 16, 16)
+    assert b200._cache_args(kv[1, 0])[1:] == (0, 0, 256, 1, 1, 4, 16, 16)
