@@ -1285,8 +1285,10 @@ int b200_paged_attention(const void* q, long long q_stride, int num_q_rows, cons
     a.scale_log2 = scale_log2;
     a.sched = static_cast<int*>(workspace);
     a.cap_items = (long long)((ws_bytes - kDecSchedBytes) / per_item);
-    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + kDecSchedBytes);
-    a.part_o = a.part_ml + (size_t)a.cap_items * Hq * 2;
+    // the 16-byte vectors first: behind an odd number of (m, l) pairs (odd
+    // Hq, odd capacity) they would not be aligned
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + kDecSchedBytes);
+    a.part_ml = a.part_o + (size_t)a.cap_items * Hq * kDecHD;
     a.out = static_cast<__nv_bfloat16*>(out); a.out_stride = out_stride;
     a.err = ds->err;
     const int smem = dec_smem_bytes();
@@ -1520,8 +1522,8 @@ extern "C" int b200_paged_decode_attention_static(
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.sched = static_cast<int*>(scratch);
   a.cap_items = (long long)((kStaticDecodeScratchBytes - kDecSchedBytes) / per_item);
-  a.part_ml = reinterpret_cast<float*>(static_cast<char*>(scratch) + kDecSchedBytes);
-  a.part_o = a.part_ml + (size_t)a.cap_items * Hq * 2;
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(scratch) + kDecSchedBytes);
+  a.part_ml = a.part_o + (size_t)a.cap_items * Hq * kDecHD;
   a.out = static_cast<__nv_bfloat16*>(out); a.out_stride = out_stride;
   a.err = ds->err;
   const int smem = dec_smem_bytes();

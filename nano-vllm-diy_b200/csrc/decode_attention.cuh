@@ -65,8 +65,8 @@ struct DecodeArgs {
   long long num_slots;
   float scale_log2;      // softmax_scale * log2(e)
   int* sched;            // workspace head (kDecSchedBytes): scheduler words, then unit counters
-  float* part_ml;        // [cap_items][Hq][2]
   float* part_o;         // [cap_items][Hq][128]
+  float* part_ml;        // [cap_items][Hq][2]
   long long cap_items;
   __nv_bfloat16* out;
   long long out_stride;
