@@ -285,6 +285,40 @@ int b200_paged_decode_attention_static(const void* q, long long q_stride, int nu
                                        int Hkv, int page, float softmax_scale, void* out,
                                        long long out_stride, b200_stream_t stream);
 
+/* Workspace of b200_shared_prefix_attention for up to `max_seqs` sequences of
+ * up to `max_seqlen_k` keys. */
+int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, size_t* bytes);
+
+/* Decode attention (one query per sequence, K/V from the paged cache) whose
+ * sequences share prefixes: what b200_paged_attention computes for
+ * max_seqlen_q == 1, with the keys of a shared prefix read once for all
+ * sequences that share it.  No counterpart in the reference, whose prefix
+ * cache (src/engine/block_manager.py:96-181) shares the blocks but not the
+ * attention over them (src/layers/attention.py:93-104).
+ *  - prefix_group: int32 [B], the group of each sequence or -1; prefix_len:
+ *    int32 [num_groups], the keys that all sequences of a group share.  The
+ *    first prefix_len / page entries of their block-table rows must be the
+ *    same (the kernel reads the first member's).  Only whole pages that every
+ *    member sees count, and a group of one shares nothing: any prefix_len
+ *    that is true of the tables is allowed.  A group outside [-1, num_groups)
+ *    counts as -1 and flags B200_DEVERR_BAD_INDEX.
+ *  - The other arguments are b200_paged_attention's.  A live sequence without
+ *    keys gives zeros; rows with q length <= 0 (padding) are left alone.
+ *  - B <= 1024, num_groups <= 1024, Hq / Hkv <= 8, page a multiple of 256,
+ *    softmax_scale > 0.
+ *  - workspace: b200_shared_prefix_workspace_bytes(B, max_seqlen_k, Hq) bytes,
+ *    256-byte aligned, its first 256 KiB + 256 bytes zero before the first
+ *    call (they are zero again after every call).  Calls that share a
+ *    workspace must not overlap on the GPU, and it is not the workspace of
+ *    b200_paged_attention. */
+int b200_shared_prefix_attention(const void* q, long long q_stride, int num_q_rows, const void* k_cache,
+                                 const void* v_cache, long long num_slots, const int* block_tables,
+                                 int bt_stride, int bt_width, const int* cu_seqlens_q,
+                                 const int* cu_seqlens_k, int B, int max_seqlen_k, int Hq, int Hkv,
+                                 int page, float softmax_scale, const int* prefix_group,
+                                 const int* prefix_len, int num_groups, void* out, long long out_stride,
+                                 void* workspace, size_t ws_bytes, b200_stream_t stream);
+
 /* Attention metadata of one step from per-sequence values, the expansion of
  * src/engine/model_runner.py:174-233 (ModelRunner.prepare_seqs) done on the
  * device.  seq_info = int32 [3][B]: start = min(num_cached_tokens, len - 1),

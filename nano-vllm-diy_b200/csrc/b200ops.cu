@@ -24,6 +24,7 @@
 #include "metadata.cuh"
 #include "pages.cuh"
 #include "prefill_tc.cuh"
+#include "shared_prefix.cuh"
 #include "gemm.cuh"
 #include "gemm_pair.cuh"
 #include "../../include/b200ops.h"
@@ -302,7 +303,7 @@ GemmPlan plan_gemm(DeviceState* ds, int T, int N, int K, bool silu_tiles) {
 // Decode attention: one CTA per SM, launched cooperatively (its merge phase
 // follows a grid-wide barrier, so every CTA must be resident).
 int launch_decode(DeviceState* ds, const CUtensorMap& tmK, const CUtensorMap& tmV,
-                  const CUtensorMap& tmQ, const DecodeArgs& a, int smem, cudaStream_t st) {
+                  const CUtensorMap& tmQ, const DecodeArgs& a, int smem, cudaStream_t st, bool shared = false) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ds->num_sms, 1, 1);
   cfg.blockDim = dim3(kDecWarps * 32, 1, 1);
@@ -313,7 +314,8 @@ int launch_decode(DeviceState* ds, const CUtensorMap& tmK, const CUtensorMap& tm
   attr[0].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_attn_kernel, tmK, tmV, tmQ, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, shared ? decode_attn_kernel<true> : decode_attn_kernel<false>, tmK,
+                                           tmV, tmQ, a);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "decode attention launch: %s", cudaGetErrorString(e));
   return B200_OK;
 }
@@ -1292,7 +1294,7 @@ int b200_paged_attention(const void* q, long long q_stride, int num_q_rows, cons
     a.out = static_cast<__nv_bfloat16*>(out); a.out_stride = out_stride;
     a.err = ds->err;
     const int smem = dec_smem_bytes();
-    if (int r = ensure_smem(ds, 2u, decode_attn_kernel, smem)) return r;
+    if (int r = ensure_smem(ds, 2u, decode_attn_kernel<false>, smem)) return r;
     if (int r = launch_decode(ds, tmK, tmV, tmQ, a, smem, st)) return r;
     return check_launch("decode_attn_kernel");
   }
@@ -1527,9 +1529,125 @@ extern "C" int b200_paged_decode_attention_static(
   a.out = static_cast<__nv_bfloat16*>(out); a.out_stride = out_stride;
   a.err = ds->err;
   const int smem = dec_smem_bytes();
-  if (int r = ensure_smem(ds, 2u, decode_attn_kernel, smem)) return r;
+  if (int r = ensure_smem(ds, 2u, decode_attn_kernel<false>, smem)) return r;
   if (int r = launch_decode(ds, tmK, tmV, tmQ, a, smem, st)) return r;
   return check_launch("decode_attn_kernel");
+}
+
+// ===========================================================================
+// Decode attention with shared prefixes (shared_prefix.cuh, decode_attention.cuh)
+// ===========================================================================
+namespace {
+
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// Bytes of the prefix part of the workspace: the sequences' records, the
+// partials of the pieces that start a row block, those of the others.
+size_t prefix_bytes(int num_sms, int seqs, int Hq) {
+  return align256(kSpRecBytes) + align256((size_t)seqs * Hq * sizeof(float2)) +
+         align256((size_t)seqs * Hq * kDecHD * sizeof(float)) +
+         align256((size_t)num_sms * kSpRows * sizeof(float2)) + (size_t)num_sms * kSpRows * kDecHD * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, size_t* bytes) {
+  if (int r = b200_attention_workspace_bytes(max_seqs, max_seqlen_k, Hq, bytes)) return r;
+  DeviceState* ds;
+  if (int r = device_state(&ds)) return r;
+  *bytes = align256(*bytes) + prefix_bytes(ds->num_sms, max_seqs, Hq);
+  return B200_OK;
+}
+
+extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, int num_q_rows, const void* k_cache,
+                                            const void* v_cache, long long num_slots, const int* block_tables,
+                                            int bt_stride, int bt_width, const int* cu_seqlens_q,
+                                            const int* cu_seqlens_k, int B, int max_seqlen_k, int Hq, int Hkv,
+                                            int page, float softmax_scale, const int* prefix_group,
+                                            const int* prefix_len, int num_groups, void* out, long long out_stride,
+                                            void* workspace, size_t ws_bytes, b200_stream_t stream) {
+  if (B <= 0) return B200_OK;
+  if (!q || !k_cache || !v_cache || !block_tables || !cu_seqlens_q || !cu_seqlens_k || !out || !prefix_group ||
+      num_groups < 0 || (num_groups > 0 && !prefix_len))
+    return fail(B200_ERR_INVALID, "shared_prefix: missing argument");
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || page <= 0 || num_q_rows <= 0 || num_slots <= 0 || max_seqlen_k < 0 ||
+      bt_width < 0 || bt_stride < 0)
+    return fail(B200_ERR_INVALID, "shared_prefix: Hq=%d Hkv=%d page=%d q rows=%d slots=%lld", Hq, Hkv, page,
+                num_q_rows, num_slots);
+  if (Hq / Hkv > 8 || Hkv > kDecMaxKvHeads || B > kSpMaxSeqs || num_groups > kSpMaxGroups || page % 256 ||
+      num_slots > 0x7fffffffLL)
+    return fail(B200_ERR_UNSUPPORTED,
+                "shared_prefix: needs Hq/Hkv <= 8, Hkv <= %d, B <= %d, groups <= %d, pages of a multiple of 256 "
+                "slots, slots in 31 bits",
+                kDecMaxKvHeads, kSpMaxSeqs, kSpMaxGroups);
+  if (!(softmax_scale > 0.f) || softmax_scale > 3e38f)
+    return fail(B200_ERR_INVALID, "shared_prefix: the scale must be positive and finite");
+  if (q_stride % 8 || out_stride % 8 || !aligned16(q) || !aligned16(out) || !aligned16(k_cache) ||
+      !aligned16(v_cache))
+    return fail(B200_ERR_INVALID, "shared_prefix: rows must be 16-byte aligned");
+  DeviceState* ds;
+  if (int r = device_state(&ds)) return r;
+  size_t need = 0;
+  if (int r = b200_shared_prefix_workspace_bytes(B, max_seqlen_k, Hq, &need)) return r;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || ws_bytes < need)
+    return fail(B200_ERR_WORKSPACE, "shared_prefix: %zu bytes of workspace (256-byte aligned) needed, %zu given", need,
+                workspace ? ws_bytes : (size_t)0);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int G = Hq / Hkv;
+  CUtensorMap tmK, tmV, tmQ;
+  const uint64_t row = (uint64_t)Hkv * kDecHD * 2;
+  DecodeArgs a{};
+  a.block_tables = block_tables; a.bt_stride = bt_stride; a.bt_width = bt_width;
+  a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = G; a.page = page; a.q_box_rows = Hq < 8 ? Hq : 8;
+  a.num_slots = num_slots;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.out = static_cast<__nv_bfloat16*>(out); a.out_stride = out_stride;
+  a.err = ds->err;
+  // workspace: the decode kernel's head and items as in b200_paged_attention, then the prefix part
+  const size_t per_item = (size_t)Hq * (kDecHD + 2) * sizeof(float);
+  char* ws = static_cast<char*>(workspace);
+  a.sched = static_cast<int*>(workspace);
+  a.cap_items = (long long)B * ((max_seqlen_k + kDecItem - 1) / kDecItem);
+  a.part_o = reinterpret_cast<float*>(ws + kDecSchedBytes);
+  a.part_ml = a.part_o + (size_t)a.cap_items * Hq * kDecHD;
+  ws += align256((size_t)kDecSchedBytes + (size_t)a.cap_items * per_item);
+  SharedArgs& s = a.sp;
+  s.q = static_cast<const __nv_bfloat16*>(q); s.q_stride = q_stride; s.num_q_rows = num_q_rows;
+  s.cu_q = cu_seqlens_q; s.cu_k = cu_seqlens_k;
+  s.block_tables = block_tables; s.bt_stride = bt_stride; s.bt_width = bt_width;
+  s.prefix_group = prefix_group; s.prefix_len = prefix_len; s.groups = num_groups;
+  s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.G = G; s.page = page; s.members = kSpRows / G;
+  s.num_slots = num_slots; s.scale_log2 = a.scale_log2;
+  s.head = reinterpret_cast<SpHead*>(ws);
+  s.rec = reinterpret_cast<SpRec*>(ws + sizeof(SpHead));
+  ws += align256(kSpRecBytes);
+  s.first_ml = reinterpret_cast<float2*>(ws);
+  ws += align256((size_t)B * Hq * sizeof(float2));
+  s.first_o = reinterpret_cast<float*>(ws);
+  ws += align256((size_t)B * Hq * kDecHD * sizeof(float));
+  s.rest_ml = reinterpret_cast<float2*>(ws);
+  ws += align256((size_t)ds->num_sms * kSpRows * sizeof(float2));
+  s.rest_o = reinterpret_cast<float*>(ws);
+  s.err = ds->err;
+  // the shared part
+  if (int r = make_tmap_3d(&tmK, k_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kSpTile)) return r;
+  if (int r = make_tmap_3d(&tmV, v_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kSpTile)) return r;
+  if (int r = ensure_smem(ds, 32u, shared_prefix_kernel, kSpSmemBytes)) return r;
+  cudaError_t e = launch_ex(shared_prefix_kernel, dim3(ds->num_sms), dim3(kSpThreads), kSpSmemBytes, st, nullptr, 0,
+                            tmK, tmV, s);
+  if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
+  if (int r = check_launch("shared_prefix_kernel")) return r;
+  // every sequence's own keys, and the merge
+  if (int r = make_tmap_3d(&tmK, k_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kDecTile)) return r;
+  if (int r = make_tmap_3d(&tmV, v_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kDecTile)) return r;
+  if (int r = make_tmap_3d(&tmQ, q, kDecHD, Hq, (uint64_t)num_q_rows, kDecHD * 2, (uint64_t)q_stride * 2, 64,
+                           (uint32_t)a.q_box_rows, 1))
+    return r;
+  const int smem = dec_smem_bytes();
+  if (int r = ensure_smem(ds, 64u, decode_attn_kernel<true>, smem)) return r;
+  if (int r = launch_decode(ds, tmK, tmV, tmQ, a, smem, st, true)) return r;
+  return check_launch("decode_attn_kernel(shared prefix)");
 }
 
 // ===========================================================================

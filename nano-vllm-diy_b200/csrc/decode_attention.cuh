@@ -30,8 +30,14 @@
 // The launch shape depends only on the SM count; context lengths are read
 // from cu_seqlens_k on the device (CUDA-graph safe; rows with q length <= 0
 // are graph padding and are skipped).
+//
+// decode_attn_kernel<true> is the second half of attention with shared
+// prefixes (shared_prefix.cuh): the items of a sequence start behind its
+// group's prefix, and the merge of a (sequence, kv head) begins with the
+// partials of the prefix.
 #pragma once
 #include "common.cuh"
+#include "shared_prefix.cuh"
 
 namespace b200 {
 
@@ -71,6 +77,7 @@ struct DecodeArgs {
   __nv_bfloat16* out;
   long long out_stride;
   unsigned* err;
+  SharedArgs sp;         // decode_attn_kernel<true> only
 };
 
 struct DecTile {
@@ -105,6 +112,7 @@ __device__ __forceinline__ uint32_t tswz(int half_bytes, int r, int ch) {
   return (uint32_t)((ch >> 3) * half_bytes + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
 }
 
+template <bool kShared>
 __global__ void __launch_bounds__(128, 1)
     decode_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                        const __grid_constant__ CUtensorMap tmQ, const DecodeArgs a) {
@@ -149,7 +157,7 @@ __global__ void __launch_bounds__(128, 1)
     int active = 0;
     for (int b = beg; b < end; ++b) {
       const int nq = a.cu_q[b + 1] - a.cu_q[b];
-      const int nk = a.cu_k[b + 1] - a.cu_k[b];
+      const int nk = a.cu_k[b + 1] - a.cu_k[b] - (kShared ? a.sp.rec[b].keys : 0);
       if (nq >= 1 && nk > 0) {
         keys += nk;
         ++active;
@@ -177,7 +185,7 @@ __global__ void __launch_bounds__(128, 1)
     int local = 0;
     for (int b = beg; b < end; ++b) {
       const int nq = a.cu_q[b + 1] - a.cu_q[b];
-      const int nk = a.cu_k[b + 1] - a.cu_k[b];
+      const int nk = a.cu_k[b + 1] - a.cu_k[b] - (kShared ? a.sp.rec[b].keys : 0);
       const int cnt = (nq >= 1 && nk > 0) ? (nk + item_len - 1) / item_len : 0;
       s_start[b] = cnt;
       local += cnt;
@@ -235,7 +243,8 @@ __global__ void __launch_bounds__(128, 1)
       if (s_start[mid] <= c) lo = mid; else hi = mid - 1;
     }
     const int b = lo;
-    const int j0 = (c - s_start[b]) * item_len;
+    const int shared = kShared ? a.sp.rec[b].keys : 0;
+    const int j0 = shared + (c - s_start[b]) * item_len;
     const int nk = a.cu_k[b + 1] - a.cu_k[b];
     const int ntok_item = min(item_len, nk - j0);
     // the block-table entries of the item's pages (one per lane 0..3)
@@ -248,7 +257,7 @@ __global__ void __launch_bounds__(128, 1)
     blk2 = __shfl_sync(0xffffffffu, e, 2);
     blk3 = __shfl_sync(0xffffffffu, e, 3);
     cur.b = b; cur.h = h; cur.c = c;
-    cur.npages = s_start[b + 1] - s_start[b];
+    cur.npages = s_start[b + 1] - s_start[b] + (shared > 0);  // > 1: parts to merge
     cur.qrow = a.cu_q[b];
     cur.ntok = ntok_item;
     cur.j0 = j0;
@@ -499,8 +508,17 @@ __global__ void __launch_bounds__(128, 1)
     if (u >= units) break;
     const int b = u / a.Hkv, h = u - b * a.Hkv;
     const int c0 = s_start[b], np = s_start[b + 1] - c0;
-    if (np <= 1) continue;  // written directly (or an empty row)
-    if (lane == 0) {
+    const bool shared = kShared && a.sp.rec[b].keys > 0;
+    if (np <= 1 && !shared) {
+      // written directly, or an empty row: no keys give zeros where a prefix
+      // could have been, padding stays as it is
+      if (kShared && np == 0 && a.cu_q[b + 1] - a.cu_q[b] >= 1)
+        for (int gg = 0; gg < a.G; ++gg)
+          *reinterpret_cast<uint2*>(a.out + (size_t)a.cu_q[b] * a.out_stride + ((size_t)h * a.G + gg) * kDecHD +
+                                    lane * 4) = make_uint2(0u, 0u);
+      continue;
+    }
+    if (lane == 0 && np > 0) {
       // the unit's items were all taken before this queue opened: wait
       // (bounded) until they are published, then zero the counter
       const unsigned long long t0 = globaltimer_ns();
@@ -522,6 +540,44 @@ __global__ void __launch_bounds__(128, 1)
       M[gg] = -INFINITY;
       L[gg] = 0.f;
       acc[gg] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if constexpr (kShared) {
+      if (shared) {
+        // the prefix: the piece that starts the row block, then those inside it
+        const SharedArgs& sp = a.sp;
+        const SpRec rc = sp.rec[b];
+        const long long u0 = rc.off + (long long)(h * rc.blocks + rc.rank / sp.members) * rc.tiles;
+        const int row0 = rc.rank % sp.members * G;
+        int p = 0, c_end = 0;
+        sp_pieces_inside(sp.head->units, sp.head->pieces, u0, rc.tiles, p, c_end);
+        const int c_begin = p;
+        for (--p; p < c_end; ++p) {
+          const bool first = p < c_begin;
+          const size_t row = first ? (size_t)b * a.Hq + (size_t)h * G : (size_t)p * kSpRows + row0;
+          const float2* ml = (first ? sp.first_ml : sp.rest_ml) + row;
+          const float* o = (first ? sp.first_o : sp.rest_o) + row * kDecHD;
+          float2 mv[8];
+          float4 ov[8];
+#pragma unroll
+          for (int gg = 0; gg < 8; ++gg) {
+            mv[gg] = gg < G ? __ldcg(ml + gg) : make_float2(-INFINITY, 0.f);
+            ov[gg] = gg < G ? __ldcg(reinterpret_cast<const float4*>(o + gg * kDecHD) + lane)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int gg = 0; gg < 8; ++gg) {
+            if (mv[gg].x == -INFINITY) continue;
+            const float mn = fmaxf(M[gg], mv[gg].x);
+            const float sc = fast_exp2(M[gg] - mn), w = fast_exp2(mv[gg].x - mn);
+            L[gg] = L[gg] * sc + w * mv[gg].y;
+            acc[gg].x = acc[gg].x * sc + w * ov[gg].x;
+            acc[gg].y = acc[gg].y * sc + w * ov[gg].y;
+            acc[gg].z = acc[gg].z * sc + w * ov[gg].z;
+            acc[gg].w = acc[gg].w * sc + w * ov[gg].w;
+            M[gg] = mn;
+          }
+        }
+      }
     }
     for (int p0 = 0; p0 < np; p0 += 2) {
       float2 ml[2][8];

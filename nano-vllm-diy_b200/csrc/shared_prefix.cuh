@@ -1,0 +1,556 @@
+// Decode attention for sequences that share a prefix: the shared part.
+//
+// The sequences of a group have the same pages at the head of their block
+// tables (prefix-cache hits, samples or beams of one prompt).  Softmax over
+// keys A + B is the combination of partials over A and over B,
+//   (m, l, o) = (max s, sum 2^(s - m), sum 2^(s - m) v),
+//   m = max(m_A, m_B), l = l_A 2^(m_A - m) + l_B 2^(m_B - m), o likewise,
+// so this kernel computes the partials of all members over the group's prefix
+// at once -- a dense product of (members x heads) query rows with the prefix
+// keys on the tensor cores, each K / V byte read once for up to 256 rows -- and
+// decode_attn_kernel<true> then streams every sequence's own keys and merges.
+//
+// Work: a unit is one 128-key tile of one row block (256 / G members of a group
+// x the G = Hq / Hkv heads of one kv head, at most 256 rows).  The units of all
+// groups, heads and blocks lie on one line that is cut into equal pieces, one
+// per CTA (one CTA per SM): no tail, whatever the groups are.  A piece that
+// starts inside a row block leaves its partial in the CTA's own slot, the
+// piece that starts the block in the rows of the sequences themselves: no
+// place is written twice, and the merge finds the pieces from the same
+// arithmetic, in a fixed order.
+//
+// Roles (10 warps): warp 0 loads K and V tiles by TMA (a ring of 32 KB slots);
+// warp 1 issues the MMAs; warps 2-5 and 6-9 are the softmax of two tiles of
+// 128 rows, one thread per row (its TMEM lane):
+//   S_t = Q_t K^T (TMEM, 128 x 128 fp32) -> registers -> P_t = 2^(s - m) as
+//   bf16 over S_t's own columns -> O_t += P_t V (P_t read from TMEM).
+// The tensor cores work on one tile while the other is in its softmax.  O_t is
+// rescaled only when the row maximum grew by more than kSpLazy (log2): P then
+// stays below 2^kSpLazy, which costs nothing in fp32 sums and in bf16's
+// relative rounding, and the rescale all but disappears after the first tile.
+// P is rounded to bf16 (the operand type of the PV product, as in the other
+// attention kernels); maxima, sums and O are fp32.
+#pragma once
+#include "common.cuh"
+#include "prefill_tc.cuh"
+
+namespace b200 {
+
+constexpr int kSpMaxSeqs = 1024;
+constexpr int kSpMaxGroups = 1024;
+constexpr int kSpRows = 256;     // rows of a block: two tiles of 128
+constexpr int kSpTile = 128;     // keys of a unit
+constexpr int kSpSlots = 4;      // ring slots of 32 KB (K, V, K, V, ...)
+constexpr int kSpThreads = 320;
+constexpr float kSpLazy = 8.f;
+constexpr int kSpQ = 0;                            // [2 tiles][2 dim halves][128 rows][128 B]
+constexpr int kSpRing = 65536;
+constexpr int kSpBar = kSpRing + kSpSlots * 32768;
+constexpr int kSpPlan = kSpBar + 256;
+
+// The groups of a call, in shared memory.
+struct SpPlan {
+  long long off[kSpMaxGroups + 1];  // first unit of each group
+  int start[kSpMaxGroups + 1];      // first member
+  int cnt[kSpMaxGroups];
+  int least[kSpMaxGroups];          // shortest member (keys)
+  int tiles[kSpMaxGroups];          // 128-key tiles of the prefix (0: nothing shared)
+  short member[kSpMaxSeqs];         // sequences by group, in batch order
+  short group[kSpMaxSeqs];
+  short rank[kSpMaxSeqs];
+};
+constexpr int kSpSmemBytes = 1024 + kSpPlan + (int)sizeof(SpPlan);
+static_assert(kSpSmemBytes <= 227 * 1024, "shared memory of one CTA");
+
+// Workspace: head {units, pieces}, one record per sequence, then the partials.
+struct SpHead {
+  long long units;
+  int pieces;
+  int pad;
+};
+struct SpRec {       // of one sequence; keys = 0: no shared part
+  int keys, tiles, blocks, rank;  // shared keys; units per row block; row blocks per kv head; member number
+  long long off;                  // the group's first unit
+  long long pad;
+};
+constexpr size_t kSpRecBytes = sizeof(SpHead) + kSpMaxSeqs * sizeof(SpRec);
+
+struct SharedArgs {
+  const __nv_bfloat16* q;
+  long long q_stride;
+  int num_q_rows;
+  const int* cu_q;
+  const int* cu_k;
+  const int* block_tables;
+  int bt_stride, bt_width;
+  const int* prefix_group;  // [B], -1: none
+  const int* prefix_len;    // [groups]
+  int groups;
+  int B, Hq, Hkv, G, page, members;  // members: of a row block, kSpRows / G
+  long long num_slots;
+  float scale_log2;
+  SpHead* head;
+  SpRec* rec;
+  float2* first_ml;   // [B * Hq]           pieces that start a row block
+  float* first_o;     // [B * Hq][128]
+  float2* rest_ml;    // [CTAs][kSpRows]    pieces that start inside one
+  float* rest_o;      // [CTAs][kSpRows][128]
+  unsigned* err;
+};
+
+// First unit of piece c.
+__host__ __device__ __forceinline__ long long sp_piece_start(long long units, int pieces, int c) {
+  return units * c / pieces;
+}
+// The pieces that start strictly inside units (u0, u0 + n): first and behind the last.
+__host__ __device__ __forceinline__ void sp_pieces_inside(long long units, int pieces, long long u0, int n, int& c0,
+                                                          int& c1) {
+  c0 = (int)(((u0 + 1) * pieces + units - 1) / units);
+  c1 = (int)(((u0 + n) * pieces + units - 1) / units);
+}
+
+__device__ __forceinline__ float sp_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 32 columns of this warp's TMEM lanes into registers that hold floats from
+// the start: nothing may touch them before tmem_ld_wait().
+__device__ __forceinline__ void sp_tmem_ld(uint32_t taddr, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(taddr));
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]: the A operand's rows are TMEM lanes, two bf16 to a column.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Builds the plan (every CTA the same) in shared memory.  All threads call it.
+__device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  for (int g = tid; g < a.groups; g += kSpThreads) {
+    s.cnt[g] = 0;
+    s.least[g] = 0x7fffffff;
+  }
+  __syncthreads();
+  for (int b = tid; b < a.B; b += kSpThreads) {
+    int g = a.prefix_group[b];
+    const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0, nk = a.cu_k[b + 1] - a.cu_k[b];
+    if (g < -1 || g >= a.groups || (nq >= 1 && (q0 < 0 || q0 >= a.num_q_rows))) {
+      if (blockIdx.x == 0) raise_error(a.err, ERR_BAD_INDEX);
+      g = -1;
+    }
+    if (nq < 1 || nk <= 0) g = -1;  // padding rows of a captured batch
+    s.group[b] = (short)g;
+    if (g >= 0) atomicMin(&s.least[g], nk);
+  }
+  __syncthreads();
+  if (tid < 32) {
+    // member numbers in batch order
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int b = b0 + lane;
+      const int g = b < a.B ? s.group[b] : -1;
+      const unsigned same = __match_any_sync(0xffffffffu, g);
+      const int before = __popc(same & ((1u << lane) - 1u));
+      int n = 0;
+      if (g >= 0) {
+        n = s.cnt[g];
+        s.rank[b] = (short)(n + before);
+      }
+      __syncwarp();
+      if (g >= 0 && before == 0) s.cnt[g] = n + __popc(same);
+      __syncwarp();
+    }
+    // prefix sums of members and units over the groups
+    int members = 0;
+    long long units = 0;
+    for (int g0 = 0; g0 < a.groups; g0 += 32) {
+      const int g = g0 + lane;
+      int n = 0, tiles = 0;
+      long long u = 0;
+      if (g < a.groups) {
+        n = s.cnt[g];
+        if (n >= 2) {
+          // whole pages that every member sees
+          int keys = min(a.prefix_len[g], s.least[g]);
+          const int pages = min(max(keys, 0) / a.page, a.bt_width);
+          tiles = pages * (a.page / kSpTile);
+        }
+        u = (long long)((n + a.members - 1) / a.members) * a.Hkv * tiles;
+      }
+      int ni = n;
+      long long ui = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, ni, o);
+        const long long y = __shfl_up_sync(0xffffffffu, ui, o);
+        if (lane >= o) {
+          ni += x;
+          ui += y;
+        }
+      }
+      if (g < a.groups) {
+        s.start[g] = members + ni - n;
+        s.off[g] = units + ui - u;
+        s.tiles[g] = tiles;
+      }
+      members += __shfl_sync(0xffffffffu, ni, 31);
+      units += __shfl_sync(0xffffffffu, ui, 31);
+    }
+    if (lane == 0) {
+      s.start[a.groups] = members;
+      s.off[a.groups] = units;
+    }
+  }
+  __syncthreads();
+  for (int b = tid; b < a.B; b += kSpThreads)
+    if (s.group[b] >= 0) s.member[s.start[s.group[b]] + s.rank[b]] = (short)b;
+  __syncthreads();
+}
+
+// A run of units of one row block.
+struct SpSeg {
+  int g, h, block;   // group, kv head, row block
+  int k0, k1;        // tiles of the prefix
+  int rows, nt;      // valid rows; tiles of 128 rows in use
+};
+
+__device__ __forceinline__ SpSeg sp_segment(const SharedArgs& a, const SpPlan& s, long long u, long long u_end) {
+  int lo = 0, hi = a.groups - 1;  // the last group that starts at u or before it
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s.off[mid] <= u) lo = mid; else hi = mid - 1;
+  }
+  SpSeg g;
+  g.g = lo;
+  const int tiles = s.tiles[lo];
+  const int n = s.start[lo + 1] - s.start[lo];
+  const int blocks = (n + a.members - 1) / a.members;
+  const long long local = u - s.off[lo];
+  const int at = (int)(local / tiles);
+  g.k0 = (int)(local - (long long)at * tiles);
+  g.h = at / blocks;
+  g.block = at - g.h * blocks;
+  const long long left = u_end - u;
+  g.k1 = left < tiles - g.k0 ? g.k0 + (int)left : tiles;
+  g.rows = min(a.members, n - g.block * a.members) * a.G;
+  g.nt = g.rows > 128 ? 2 : 1;
+  return g;
+}
+
+// First cache row of tile k of the group's prefix, from its first member's table; -1: no such page.
+__device__ __forceinline__ long long sp_tile_row(const SharedArgs& a, int leader, int k) {
+  const int per = a.page / kSpTile;
+  const int col = k / per;
+  const long long blk = a.block_tables[(size_t)leader * a.bt_stride + col];
+  const long long row = blk * a.page + (long long)(k - col * per) * kSpTile;
+  return blk >= 0 && row + kSpTile <= a.num_slots ? row : -1;
+}
+
+__global__ void __launch_bounds__(kSpThreads, 1)
+    shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                         const SharedArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSpBar);
+  uint64_t* full = bars;                   // [kSpSlots]
+  uint64_t* empty = bars + kSpSlots;       // [kSpSlots]
+  uint64_t* q_full = bars + 2 * kSpSlots;  // [2] a segment's query rows are in shared memory, O may be overwritten
+  uint64_t* s_full = q_full + 2;           // [2]
+  uint64_t* p_full = q_full + 4;           // [2]
+  uint64_t* o_done = q_full + 6;           // [2]
+  uint64_t* drain = q_full + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 9);
+  SpPlan& plan = *reinterpret_cast<SpPlan*>(smem + kSpPlan);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    for (int i = 0; i < 2 * kSpSlots; ++i) mbar_init(&bars[i], 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 4);  // a warp's lane 0 arrives for its rows
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_done[t], 1);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  sp_build_plan(a, plan);
+  const long long units = plan.off[a.groups];
+  const int pieces = (int)(units < gridDim.x ? units : gridDim.x);
+  if (blockIdx.x == 0) {
+    // what the merge needs
+    if (threadIdx.x == 0) {
+      a.head->units = units;
+      a.head->pieces = pieces;
+    }
+    for (int b = threadIdx.x; b < a.B; b += kSpThreads) {
+      SpRec r{};
+      const int g = plan.group[b];
+      if (g >= 0 && plan.tiles[g] > 0) {
+        r.keys = plan.tiles[g] * kSpTile;
+        r.tiles = plan.tiles[g];
+        r.blocks = (plan.start[g + 1] - plan.start[g] + a.members - 1) / a.members;
+        r.rank = plan.rank[b];
+        r.off = plan.off[g];
+      }
+      a.rec[b] = r;
+    }
+  }
+  if ((int)blockIdx.x >= pieces) return;  // the whole CTA, before any TMEM
+  const long long u_beg = sp_piece_start(units, pieces, blockIdx.x);
+  const long long u_end = sp_piece_start(units, pieces, blockIdx.x + 1);
+
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // S / P of tile t at t * 128, O of tile t at 256 + t * 128
+  const uint32_t base = smem_u32(smem);
+
+  if (warp == 0) {
+    // ---- producer
+    if (lane == 0) {
+      int it = 0;      // loads issued; load it is in slot it % kSpSlots
+      bool ok = true;
+      for (long long u = u_beg; ok && u < u_end;) {
+        const SpSeg g = sp_segment(a, plan, u, u_end);
+        const int leader = plan.member[plan.start[g.g]];
+        for (int k = g.k0; ok && k < g.k1; ++k) {
+          long long row = sp_tile_row(a, leader, k);
+          if (row < 0) {
+            raise_error(a.err, ERR_BAD_INDEX);
+            row = a.num_slots;  // behind the cache: the load fills zeros (the softmax masks the tile)
+          }
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const int sl = it % kSpSlots;
+            if (it >= kSpSlots && !mbar_wait(&empty[sl], (uint32_t)(it / kSpSlots + 1) & 1u, a.err)) {
+              ok = false;
+              break;
+            }
+            const uint32_t dst = base + kSpRing + (uint32_t)sl * 32768u, bar = smem_u32(&full[sl]);
+            mbar_arrive_expect_tx(&full[sl], 32768);
+            tma_load_3d(dst, kv ? &tmV : &tmK, bar, 0, g.h, (int)row);
+            tma_load_3d(dst + 16384, kv ? &tmV : &tmK, bar, 64, g.h, (int)row);
+            ++it;
+          }
+        }
+        u += g.k1 - g.k0;
+      }
+      // every load has landed before the CTA may end (a wait that gave up leaves some unread)
+      for (int i = it > kSpSlots ? it - kSpSlots : 0; i < it; ++i)
+        mbar_wait(&full[i % kSpSlots], (uint32_t)(i / kSpSlots) & 1u, a.err);
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer
+    if (lane == 0) {
+      const uint32_t idesc_s = umma_idesc_bf16(128, kSpTile);
+      const uint32_t idesc_o = umma_idesc_bf16(128, 128) | (1u << 16);  // B (V) MN-major
+      int it = 0, seg[2] = {0, 0}, step[2] = {0, 0};
+      bool ok = true;
+      auto wait_slot = [&](int i) { return mbar_wait(&full[i % kSpSlots], (uint32_t)(i / kSpSlots) & 1u, a.err); };
+      auto scores = [&](int t, int i) {  // S_t = Q_t K^T, K in load i
+        const uint32_t qb = base + kSpQ + (uint32_t)t * 32768u;
+        const uint32_t kb = base + kSpRing + (uint32_t)(i % kSpSlots) * 32768u;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const uint32_t o = (uint32_t)(kk >> 2) * 16384u + (uint32_t)(kk & 3) * 32u;
+          tc_mma_f16(tmem + (uint32_t)t * 128u, umma_desc_sw128(qb + o), umma_desc_sw128(kb + o), idesc_s,
+                     kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&s_full[t]);
+      };
+      auto values = [&](int t, int i, bool acc) {  // O_t (+)= P_t V, V in load i
+        const uint32_t vb = base + kSpRing + (uint32_t)(i % kSpSlots) * 32768u;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          tc_mma_f16_ts(tmem + 256u + (uint32_t)t * 128u, tmem + (uint32_t)t * 128u + (uint32_t)kk * 8u,
+                        umma_desc_sw128_mn(vb + (uint32_t)kk * 2048u, 16384u), idesc_o, (acc || kk > 0) ? 1u : 0u);
+      };
+      for (long long u = u_beg; ok && u < u_end;) {
+        const SpSeg g = sp_segment(a, plan, u, u_end);
+        // the first scores of both tiles
+        if (!wait_slot(it)) break;
+        for (int t = 0; ok && t < g.nt; ++t) {
+          ok = mbar_wait(&q_full[t], (uint32_t)seg[t] & 1u, a.err);
+          tc_fence_after();
+          if (ok) scores(t, it);
+        }
+        if (!ok) break;
+        tc_commit(&empty[it % kSpSlots]);
+        for (int k = g.k0; ok && k < g.k1; ++k, it += 2) {
+          const bool more = k + 1 < g.k1;
+          ok = wait_slot(it + 1) && (!more || wait_slot(it + 2));
+          for (int t = 0; ok && t < g.nt; ++t) {
+            ok = mbar_wait(&p_full[t], (uint32_t)step[t] & 1u, a.err);
+            if (!ok) break;
+            ++step[t];
+            tc_fence_after();
+            values(t, it + 1, k > g.k0);
+            // S_t's next scores overwrite P_t: MMAs of one thread run in the order of issue
+            if (more) scores(t, it + 2);
+            else tc_commit(&o_done[t]);
+          }
+          if (!ok) break;
+          tc_commit(&empty[(it + 1) % kSpSlots]);
+          if (more) tc_commit(&empty[(it + 2) % kSpSlots]);
+        }
+        for (int t = 0; t < g.nt; ++t) ++seg[t];
+        u += g.k1 - g.k0;
+      }
+      // every MMA issued has completed before TMEM can be released
+      tc_commit(drain);
+      mbar_wait(drain, 0u, a.err);
+    }
+  } else {
+    // ---- softmax: one thread per row of its tile
+    const int t = warp >= 6;
+    const int q4 = warp & 3;             // TMEM lane quarter of this warp
+    const int row = q4 * 32 + lane;      // of the tile
+    const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+    const uint32_t ts = tmem + lanes + (uint32_t)t * 128u, to = ts + 256u;
+    int seg = 0, step = 0;
+    bool ok = true;
+    for (long long u = u_beg; ok && u < u_end;) {
+      const SpSeg g = sp_segment(a, plan, u, u_end);
+      u += g.k1 - g.k0;
+      if (t >= g.nt) continue;
+      const int r = t * 128 + row;  // row of the block: member r / G, head r % G
+      const bool valid = r < g.rows;
+      const int m0 = plan.start[g.g] + g.block * a.members;
+      const int b = plan.member[valid ? m0 + r / a.G : m0];
+      const int hq = g.h * a.G + r % a.G;
+      {
+        // the row's 128 dims in the swizzled K-major layout of the MMA (zeros behind the last member)
+        uint8_t* dst = smem + kSpQ + t * 32768 + row * 128;
+        const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)a.cu_q[b] * a.q_stride + hq * 128);
+        uint4 v[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c] = valid ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = v[c];
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[t]);
+      }
+      const int leader = plan.member[plan.start[g.g]];
+      float m = -INFINITY, l = 0.f;
+      for (int k = g.k0; ok && k < g.k1; ++k, ++step) {
+        ok = mbar_wait(&s_full[t], (uint32_t)step & 1u, a.err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sp_tmem_ld(ts + (uint32_t)(c * 32), s + c * 32);
+        tmem_ld_wait();
+        // every use of s stays behind the wait
+#pragma unroll
+        for (int i = 0; i < 128; ++i) asm volatile("" : "+f"(s[i]));
+        const bool there = sp_tile_row(a, leader, k) >= 0;
+        float mt = s[0];
+#pragma unroll
+        for (int i = 1; i < 128; ++i) mt = fmaxf(mt, s[i]);
+        mt = there ? mt * a.scale_log2 : -INFINITY;
+        if (!there) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) s[i] = -INFINITY;
+        }
+        // S complete means that O_t += P V of the tile before is too: rescale O in place
+        if (__any_sync(0xffffffffu, mt > m + kSpLazy)) {
+          const float m_new = fmaxf(m, mt);
+          const float alpha = m == -INFINITY ? 0.f : sp_exp2(m - m_new);
+          if (k > g.k0) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t x[32];
+              tmem_ld_32x32b_x32(to + (uint32_t)(c * 32), x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+              tmem_st_32x32b_x32(to + (uint32_t)(c * 32), x);
+            }
+          }
+          l *= alpha;
+          m = m_new;
+        }
+        const float mm = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: P = 0
+        float rs = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float p0 = sp_exp2(fmaf(s[c * 64 + 2 * i], a.scale_log2, -mm));
+            const float p1 = sp_exp2(fmaf(s[c * 64 + 2 * i + 1], a.scale_log2, -mm));
+            rs += p0 + p1;
+            pk[i] = pack_bf16x2(p0, p1);
+          }
+          tmem_st_32x32b_x32(ts + (uint32_t)(c * 32), pk);
+        }
+        l += rs;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      // ---- the segment's partial
+      ok = mbar_wait(&o_done[t], (uint32_t)seg & 1u, a.err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      ++seg;
+      tc_fence_after();
+      const bool first = g.k0 == 0;
+      const size_t at = first ? (size_t)b * a.Hq + hq : (size_t)blockIdx.x * kSpRows + r;
+      float* po = (first ? a.first_o : a.rest_o) + at * 128;
+      if (valid) (first ? a.first_ml : a.rest_ml)[at] = make_float2(m, l);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[32];
+        tmem_ld_32x32b_x32(to + (uint32_t)(c * 32), x);
+        tmem_ld_wait();
+        if (valid) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(po + c * 32 + i) =
+                make_float4(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]),
+                            __uint_as_float(x[i + 3]));
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace b200

@@ -72,6 +72,10 @@ _SIGNATURES = {
                                     ctypes.c_ulonglong, ctypes.c_ulonglong, _c_void_p, _c_void_p], _i),
     "b200_select_tokens_exchange": ([_c_void_p, _i, _i, _i, _c_void_p, _c_void_p, _c_void_p, _ll,
                                      _c_void_p, _c_void_p], _i),
+    "b200_shared_prefix_workspace_bytes": ([_i, _i, _i, ctypes.POINTER(_sz)], _i),
+    "b200_shared_prefix_attention": ([_c_void_p, _ll, _i, _c_void_p, _c_void_p, _ll, _c_void_p, _i, _i,
+                                      _c_void_p, _c_void_p, _i, _i, _i, _i, _i, _f, _c_void_p,
+                                      _c_void_p, _i, _c_void_p, _ll, _c_void_p, _sz, _c_void_p], _i),
     "b200_copy_pages": ([_c_void_p, _ll, _ll, _ll, _i, _i, _i, _i, _ll, _c_void_p, _c_void_p,
                          _c_void_p, _i, _c_void_p], _i),
     "b200_take_pages": ([_c_void_p, _ll, _i, _i, _c_void_p, _c_void_p, _i, _i, _c_void_p, _c_void_p,
@@ -140,6 +144,34 @@ def _bf16(*ts: torch.Tensor | None) -> None:
             raise TypeError(f"expected bfloat16, got {t.dtype}")
 
 
+_SAME = contextlib.nullcontext()
+
+
+def _device_of(*ts: torch.Tensor | None):
+    """A context in which the current device (and so the current stream) is
+    that of the tensors, which must all be on one."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("b200 kernels need CUDA tensors (there is no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return _SAME if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _index(name: str, t: torch.Tensor, n: int | None = None) -> int:
+    """Entries of an int32 vector the kernels index as t[i]."""
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32")
+    if t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1) or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} must be a contiguous vector" + (f" of {n}" if n is not None else ""))
+    return t.shape[0]
+
+
 def _rows(t: torch.Tensor) -> tuple[int, int]:
     """(rows, row_stride) of a tensor whose last dim is contiguous and whose
     leading dims collapse into uniformly strided rows."""
@@ -159,6 +191,7 @@ def _rows(t: torch.Tensor) -> tuple[int, int]:
 # workspaces
 # ---------------------------------------------------------------------------
 _workspaces: dict[tuple[int, str], torch.Tensor] = {}
+_outgrown: list[torch.Tensor] = []  # kept: graphs captured with them still write there
 
 
 def workspace(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
@@ -171,6 +204,8 @@ def workspace(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"workspace '{kind}' must be sized before CUDA-graph capture "
                                f"({nbytes} bytes requested)")
+        if buf is not None:
+            _outgrown.append(buf)
         buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _workspaces[key] = buf
     return buf
@@ -202,7 +237,8 @@ def device_error(clear: bool = True) -> int:
     _check(load_library().b200_device_error(ctypes.byref(v), int(clear)), "b200_device_error")
     if clear and v.value & _TIMEOUT_BITS:
         dev = torch.cuda.current_device()
-        heads = {"attn": attention_workspace_bytes(0, 0, 1), "gemm": _GEMM_FLAG_BYTES}
+        head = attention_workspace_bytes(0, 0, 1)
+        heads = {"attn": head, "shared_prefix": head, "gemm": _GEMM_FLAG_BYTES}
         for (d, kind), buf in _workspaces.items():
             if d == dev and kind in heads:
                 buf[:heads[kind]].zero_()
@@ -569,37 +605,69 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | N
     return out
 
 
+_prefix_ws_bytes: dict[tuple[int, int, int, int], int] = {}
+
+
+def shared_prefix_workspace_bytes(max_seqs: int, max_seqlen_k: int, num_heads: int) -> int:
+    """(of the current device: its size depends on the SM count)"""
+    key = (torch.cuda.current_device(), max_seqs, max_seqlen_k, num_heads)
+    n = _prefix_ws_bytes.get(key)
+    if n is None:
+        size = ctypes.c_size_t(0)
+        _check(load_library().b200_shared_prefix_workspace_bytes(max_seqs, max_seqlen_k, num_heads,
+                                                                 ctypes.byref(size)),
+               "b200_shared_prefix_workspace_bytes")
+        if len(_prefix_ws_bytes) > 4096:
+            _prefix_ws_bytes.clear()
+        n = _prefix_ws_bytes[key] = int(size.value)
+    return n
+
+
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, max_seqlen_k: int,
+                            softmax_scale: float, block_table: torch.Tensor, prefix_group: torch.Tensor,
+                            prefix_len: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_attention of a decode batch (one query per sequence) whose sequences share prefixes.
+
+    prefix_group int32 [B]: the group of each sequence, -1 for none; prefix_len int32 [groups]: the
+    keys shared in each group, that is, the first prefix_len // page pages of the block tables of its
+    sequences are the same (src.engine.metadata.shared_prefixes finds such groups).  The keys of a
+    prefix are read once for its whole group."""
+    with _device_of(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, prefix_group, prefix_len, out):
+        _bf16(q, k_cache, v_cache, out)
+        B = _index("cu_seqlens_q", cu_seqlens_q) - 1
+        _index("cu_seqlens_k", cu_seqlens_k, B + 1)
+        _index("prefix_group", prefix_group, B)
+        groups = _index("prefix_len", prefix_len)
+        T, Hq, D = q.shape
+        if D != 128 or k_cache.dim() != 4 or k_cache.shape[3] != 128:
+            raise ValueError("head_dim must be 128 and the caches [pages, page, kv heads, 128]")
+        if v_cache.shape != k_cache.shape or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+            raise ValueError("k_cache and v_cache must be contiguous and of one shape")
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+            raise TypeError("block_table must be int32 [B, width] with contiguous rows")
+        if block_table.shape[0] != B:
+            raise ValueError(f"block_table of {block_table.shape[0]} rows for {B} sequences")
+        if q.stride(-1) != 1 or q.stride(1) != 128:
+            q = q.contiguous()
+        if out is None:
+            out = torch.empty(T, Hq, 128, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.stride(-1) != 1 or out.stride(1) != 128:
+            raise ValueError(f"out must be {tuple(q.shape)} with contiguous heads")
+        pages, page, Hkv, _ = k_cache.shape
+        ws = workspace("shared_prefix", shared_prefix_workspace_bytes(B, int(max_seqlen_k), Hq), q.device)
+        _check(load_library().b200_shared_prefix_attention(
+            q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), pages * page,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cu_seqlens_q.data_ptr(),
+            cu_seqlens_k.data_ptr(), B, int(max_seqlen_k), Hq, Hkv, page, float(softmax_scale),
+            prefix_group.data_ptr(), prefix_len.data_ptr(), groups, out.data_ptr(), out.stride(0),
+            ws.data_ptr(), ws.numel(), _stream()), "b200_shared_prefix_attention")
+    return out
+
+
 # ---------------------------------------------------------------------------
 # pages of the KV cache
 # ---------------------------------------------------------------------------
-_SAME = contextlib.nullcontext()
-
-
-def _device_of(*ts: torch.Tensor | None):
-    """A context in which the current device (and so the current stream) is
-    that of the tensors, which must all be on one."""
-    dev = None
-    for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("b200 kernels need CUDA tensors (there is no CPU path)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return _SAME if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _index(name: str, t: torch.Tensor, n: int | None = None) -> int:
-    """Entries of an int32 vector the kernels index as t[i]."""
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} must be int32")
-    if t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1) or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name} must be a contiguous vector" + (f" of {n}" if n is not None else ""))
-    return t.shape[0]
-
-
 def _cache_args(kv_cache: torch.Tensor):
     """C arguments of a cache [pages, page, Hkv, D] with up to two leading plane
     dimensions (the runner's [2, layers, pages, page, Hkv, D]) and contiguous pages."""

@@ -192,3 +192,35 @@ def test_page_operators_refuse_cpu_tensors_types_and_layouts():
     # planes and their strides, in bytes
     assert b200._cache_args(kv)[1:] == (1024, 1024, 256, 2, 1, 4, 16, 16)
     assert b200._cache_args(kv[1, 0])[1:] == (0, 0, 256, 1, 1, 4, 16, 16)
+
+
+def test_shared_prefix_attention_refuses_before_any_launch():
+    from src import b200
+    lib = b200.load_library()
+    p = ctypes.c_void_p(256)
+    good = [p, 1024, 4, p, p, 2560, p, 8, 8, p, p, 4, 2048, 8, 2, 256, 0.1, p, p, 1, p, 1024, p, 1 << 30, None]
+    names = ("q q_stride rows k v slots bt bt_stride bt_width cu_q cu_k B max_k Hq Hkv page scale group len groups out "
+             "out_stride ws ws_bytes stream").split()
+
+    def call(**kw):
+        return lib.b200_shared_prefix_attention(*[kw.get(n, v) for n, v in zip(names, good)])
+
+    assert call(B=0) == 0
+    for kw in (dict(q=None), dict(group=None), dict(len=None), dict(bt=None), dict(groups=-1), dict(Hq=9),
+               dict(rows=0), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")), dict(scale=float("inf")),
+               dict(q_stride=1028), dict(out=ctypes.c_void_p(264)), dict(k=ctypes.c_void_p(8)), dict(max_k=-1)):
+        assert call(**kw) == -1, kw
+    for kw in (dict(Hq=18, Hkv=2), dict(B=1025), dict(groups=1025), dict(page=128), dict(Hq=65, Hkv=65),
+               dict(slots=1 << 31)):
+        assert call(**kw) == -2, kw
+
+
+def test_shared_prefix_attention_refuses_cpu_tensors():
+    import pytest
+    import torch
+    from src import b200
+    q = torch.zeros(2, 2, 128, dtype=torch.bfloat16)
+    c = torch.zeros(2, 256, 1, 128, dtype=torch.bfloat16)
+    i = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        b200.shared_prefix_attention(q, c, c, i, i, 4, 0.1, torch.zeros(2, 1, dtype=torch.int32), i[:2], i[:1])
