@@ -287,7 +287,7 @@ int b200_paged_decode_attention_static(const void* q, long long q_stride, int nu
 
 /* Workspace of b200_shared_prefix_attention for up to `max_seqs` sequences of
  * up to `max_seqlen_k` keys. */
-int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, size_t* bytes);
+int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, int Hkv, size_t* bytes);
 
 /* Decode attention (one query per sequence, K/V from the paged cache) whose
  * sequences share prefixes: what b200_paged_attention computes for
@@ -306,7 +306,7 @@ int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, s
  *    keys gives zeros; rows with q length <= 0 (padding) are left alone.
  *  - B <= 1024, num_groups <= 1024, Hq / Hkv <= 8, page a multiple of 256,
  *    softmax_scale > 0.
- *  - workspace: b200_shared_prefix_workspace_bytes(B, max_seqlen_k, Hq) bytes,
+ *  - workspace: b200_shared_prefix_workspace_bytes(B, max_seqlen_k, Hq, Hkv) bytes,
  *    256-byte aligned, its first 256 KiB + 256 bytes zero before the first
  *    call (they are zero again after every call).  Calls that share a
  *    workspace must not overlap on the GPU, and it is not the workspace of

@@ -303,7 +303,7 @@ GemmPlan plan_gemm(DeviceState* ds, int T, int N, int K, bool silu_tiles) {
 // Decode attention: one CTA per SM, launched cooperatively (its merge phase
 // follows a grid-wide barrier, so every CTA must be resident).
 int launch_decode(DeviceState* ds, const CUtensorMap& tmK, const CUtensorMap& tmV,
-                  const CUtensorMap& tmQ, const DecodeArgs& a, int smem, cudaStream_t st, bool shared = false) {
+                  const CUtensorMap& tmQ, const DecodeArgs& a, int smem, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ds->num_sms, 1, 1);
   cfg.blockDim = dim3(kDecWarps * 32, 1, 1);
@@ -314,8 +314,7 @@ int launch_decode(DeviceState* ds, const CUtensorMap& tmK, const CUtensorMap& tm
   attr[0].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, shared ? decode_attn_kernel<true> : decode_attn_kernel<false>, tmK,
-                                           tmV, tmQ, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_attn_kernel<false>, tmK, tmV, tmQ, a);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "decode attention launch: %s", cudaGetErrorString(e));
   return B200_OK;
 }
@@ -1541,21 +1540,65 @@ namespace {
 
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
-// Bytes of the prefix part of the workspace: the sequences' records, the
-// partials of the pieces that start a row block, those of the others.
-size_t prefix_bytes(int num_sms, int seqs, int Hq) {
-  return align256(kSpRecBytes) + align256((size_t)seqs * Hq * sizeof(float2)) +
-         align256((size_t)seqs * Hq * kDecHD * sizeof(float)) +
-         align256((size_t)num_sms * kSpRows * sizeof(float2)) + (size_t)num_sms * kSpRows * kDecHD * sizeof(float);
+// Items (of the sequences' own keys) the workspace has room for: 512 keys each
+// and one more per sequence, or as many short ones as there are warps.
+long long shared_items(int num_sms, int seqs, int max_seqlen_k, int Hkv) {
+  return (long long)seqs * ((max_seqlen_k + kDecItem - 1) / kDecItem + 1) +
+         ((long long)num_sms * kDecWarps + Hkv - 1) / Hkv;
+}
+
+// The workspace: the decode kernel's head and items, the sequences' records
+// and first items, the partials of the pieces that start a row block, those of
+// the others.
+struct SharedLayout {
+  size_t part_o, part_ml, head, starts, first_ml, first_o, rest_ml, rest_o, total;
+};
+SharedLayout shared_layout(int num_sms, int seqs, int max_seqlen_k, int Hq, int Hkv) {
+  const size_t items = (size_t)shared_items(num_sms, seqs, max_seqlen_k, Hkv), rows = (size_t)seqs * Hq,
+               rest = (size_t)num_sms * kSpRows;
+  SharedLayout l{};
+  size_t at = align256(kDecSchedBytes);
+  auto take = [&](size_t bytes) {
+    const size_t from = at;
+    at += align256(bytes);
+    return from;
+  };
+  l.part_o = take(items * Hq * kDecHD * sizeof(float));
+  l.part_ml = take(items * Hq * sizeof(float2));
+  l.head = take(kSpRecBytes);
+  l.starts = take((kSpMaxSeqs + 1) * sizeof(int));
+  l.first_ml = take(rows * sizeof(float2));
+  l.first_o = take(rows * kDecHD * sizeof(float));
+  l.rest_ml = take(rest * sizeof(float2));
+  l.rest_o = take(rest * kDecHD * sizeof(float));
+  l.total = at;
+  return l;
+}
+
+// Launch that may begin while the one before it in the stream still runs (see griddep_wait).
+template <typename... KArgs, typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 }  // namespace
 
-extern "C" int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, size_t* bytes) {
-  if (int r = b200_attention_workspace_bytes(max_seqs, max_seqlen_k, Hq, bytes)) return r;
+extern "C" int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, int Hkv, size_t* bytes) {
+  if (!bytes || max_seqs < 0 || max_seqlen_k < 0 || Hq <= 0 || Hkv <= 0 || Hkv > Hq)
+    return fail(B200_ERR_INVALID, "bad arguments");
   DeviceState* ds;
   if (int r = device_state(&ds)) return r;
-  *bytes = align256(*bytes) + prefix_bytes(ds->num_sms, max_seqs, Hq);
+  *bytes = shared_layout(ds->num_sms, max_seqs, max_seqlen_k, Hq, Hkv).total;
   return B200_OK;
 }
 
@@ -1587,11 +1630,10 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
     return fail(B200_ERR_INVALID, "shared_prefix: rows must be 16-byte aligned");
   DeviceState* ds;
   if (int r = device_state(&ds)) return r;
-  size_t need = 0;
-  if (int r = b200_shared_prefix_workspace_bytes(B, max_seqlen_k, Hq, &need)) return r;
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || ws_bytes < need)
-    return fail(B200_ERR_WORKSPACE, "shared_prefix: %zu bytes of workspace (256-byte aligned) needed, %zu given", need,
-                workspace ? ws_bytes : (size_t)0);
+  const SharedLayout l = shared_layout(ds->num_sms, B, max_seqlen_k, Hq, Hkv);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || ws_bytes < l.total)
+    return fail(B200_ERR_WORKSPACE, "shared_prefix: %zu bytes of workspace (256-byte aligned) needed, %zu given",
+                l.total, workspace ? ws_bytes : (size_t)0);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int G = Hq / Hkv;
   CUtensorMap tmK, tmV, tmQ;
@@ -1604,14 +1646,11 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.out = static_cast<__nv_bfloat16*>(out); a.out_stride = out_stride;
   a.err = ds->err;
-  // workspace: the decode kernel's head and items as in b200_paged_attention, then the prefix part
-  const size_t per_item = (size_t)Hq * (kDecHD + 2) * sizeof(float);
   char* ws = static_cast<char*>(workspace);
   a.sched = static_cast<int*>(workspace);
-  a.cap_items = (long long)B * ((max_seqlen_k + kDecItem - 1) / kDecItem);
-  a.part_o = reinterpret_cast<float*>(ws + kDecSchedBytes);
-  a.part_ml = a.part_o + (size_t)a.cap_items * Hq * kDecHD;
-  ws += align256((size_t)kDecSchedBytes + (size_t)a.cap_items * per_item);
+  a.cap_items = shared_items(ds->num_sms, B, max_seqlen_k, Hkv);
+  a.part_o = reinterpret_cast<float*>(ws + l.part_o);
+  a.part_ml = reinterpret_cast<float*>(ws + l.part_ml);
   SharedArgs& s = a.sp;
   s.q = static_cast<const __nv_bfloat16*>(q); s.q_stride = q_stride; s.num_q_rows = num_q_rows;
   s.cu_q = cu_seqlens_q; s.cu_k = cu_seqlens_k;
@@ -1619,16 +1658,13 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   s.prefix_group = prefix_group; s.prefix_len = prefix_len; s.groups = num_groups;
   s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.G = G; s.page = page; s.members = kSpRows / G;
   s.num_slots = num_slots; s.scale_log2 = a.scale_log2;
-  s.head = reinterpret_cast<SpHead*>(ws);
-  s.rec = reinterpret_cast<SpRec*>(ws + sizeof(SpHead));
-  ws += align256(kSpRecBytes);
-  s.first_ml = reinterpret_cast<float2*>(ws);
-  ws += align256((size_t)B * Hq * sizeof(float2));
-  s.first_o = reinterpret_cast<float*>(ws);
-  ws += align256((size_t)B * Hq * kDecHD * sizeof(float));
-  s.rest_ml = reinterpret_cast<float2*>(ws);
-  ws += align256((size_t)ds->num_sms * kSpRows * sizeof(float2));
-  s.rest_o = reinterpret_cast<float*>(ws);
+  s.head = reinterpret_cast<SpHead*>(ws + l.head);
+  s.rec = reinterpret_cast<SpRec*>(ws + l.head + sizeof(SpHead));
+  s.starts = reinterpret_cast<int*>(ws + l.starts);
+  s.first_ml = reinterpret_cast<float2*>(ws + l.first_ml);
+  s.first_o = reinterpret_cast<float*>(ws + l.first_o);
+  s.rest_ml = reinterpret_cast<float2*>(ws + l.rest_ml);
+  s.rest_o = reinterpret_cast<float*>(ws + l.rest_o);
   s.err = ds->err;
   // the shared part
   if (int r = make_tmap_3d(&tmK, k_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kSpTile)) return r;
@@ -1638,16 +1674,21 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
                             tmK, tmV, s);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
   if (int r = check_launch("shared_prefix_kernel")) return r;
-  // every sequence's own keys, and the merge
+  // every sequence's own keys
   if (int r = make_tmap_3d(&tmK, k_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kDecTile)) return r;
   if (int r = make_tmap_3d(&tmV, v_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kDecTile)) return r;
   if (int r = make_tmap_3d(&tmQ, q, kDecHD, Hq, (uint64_t)num_q_rows, kDecHD * 2, (uint64_t)q_stride * 2, 64,
                            (uint32_t)a.q_box_rows, 1))
     return r;
-  const int smem = dec_smem_bytes();
+  const int smem = dec_smem_bytes<true>();
   if (int r = ensure_smem(ds, 64u, decode_attn_kernel<true>, smem)) return r;
-  if (int r = launch_decode(ds, tmK, tmV, tmQ, a, smem, st, true)) return r;
-  return check_launch("decode_attn_kernel(shared prefix)");
+  e = launch_overlapped(decode_attn_kernel<true>, ds->num_sms, kDecWarps * 32, smem, st, tmK, tmV, tmQ, a);
+  if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
+  if (int r = check_launch("decode_attn_kernel(shared prefix)")) return r;
+  // the parts of each row
+  e = launch_overlapped(shared_merge_kernel, (B * Hq + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, st, a);
+  if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
+  return check_launch("shared_merge_kernel");
 }
 
 // ===========================================================================

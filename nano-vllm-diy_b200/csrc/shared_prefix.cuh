@@ -7,7 +7,7 @@
 //   m = max(m_A, m_B), l = l_A 2^(m_A - m) + l_B 2^(m_B - m), o likewise,
 // so this kernel computes the partials of all members over the group's prefix
 // at once -- a dense product of (members x heads) query rows with the prefix
-// keys on the tensor cores, each K / V byte read once for up to 256 rows -- and
+// keys on the tensor cores, each K / V byte read once for up to 256 rows --,
 // decode_attn_kernel<true> then streams every sequence's own keys and merges.
 //
 // Work: a unit is one 128-key tile of one row block (256 / G members of a group
@@ -19,9 +19,11 @@
 // place is written twice, and the merge finds the pieces from the same
 // arithmetic, in a fixed order.
 //
-// Roles (10 warps): warp 0 loads K and V tiles by TMA (a ring of 32 KB slots);
-// warp 1 issues the MMAs; warps 2-5 and 6-9 are the softmax of two tiles of
-// 128 rows, one thread per row (its TMEM lane):
+// Roles (three warpgroups): warp 0 loads K and V tiles by TMA (a ring of 32 KB
+// slots), warp 1 issues the MMAs (warps 2 and 3 only complete their
+// warpgroup, which gives most of its registers away); warps 4-7 and 8-11 are
+// the softmax of two tiles of 128 rows, one thread per row (its TMEM lane),
+// whose 128 scores stay in registers:
 //   S_t = Q_t K^T (TMEM, 128 x 128 fp32) -> registers -> P_t = 2^(s - m) as
 //   bf16 over S_t's own columns -> O_t += P_t V (P_t read from TMEM).
 // The tensor cores work on one tile while the other is in its softmax.  O_t is
@@ -41,7 +43,11 @@ constexpr int kSpMaxGroups = 1024;
 constexpr int kSpRows = 256;     // rows of a block: two tiles of 128
 constexpr int kSpTile = 128;     // keys of a unit
 constexpr int kSpSlots = 4;      // ring slots of 32 KB (K, V, K, V, ...)
-constexpr int kSpThreads = 320;
+constexpr int kSpThreads = 384;
+// registers: 168 a thread at launch (64 K over 12 warps), then 88 for the first
+// warpgroup and 208 for the softmax: 128 x (88 + 208 + 208) = 384 x 168
+constexpr int kSpRegsLaunch = 168, kSpRegsIssue = 88, kSpRegsSoftmax = 208;
+static_assert(kSpRegsIssue + 2 * kSpRegsSoftmax == 3 * kSpRegsLaunch, "the shares are what the launch has");
 constexpr float kSpLazy = 8.f;
 constexpr int kSpQ = 0;                            // [2 tiles][2 dim halves][128 rows][128 B]
 constexpr int kSpRing = 65536;
@@ -71,7 +77,7 @@ struct SpHead {
 struct SpRec {       // of one sequence; keys = 0: no shared part
   int keys, tiles, blocks, rank;  // shared keys; units per row block; row blocks per kv head; member number
   long long off;                  // the group's first unit
-  long long pad;
+  int start, members;             // members of the groups before; members of the group
 };
 constexpr size_t kSpRecBytes = sizeof(SpHead) + kSpMaxSeqs * sizeof(SpRec);
 
@@ -91,9 +97,10 @@ struct SharedArgs {
   float scale_log2;
   SpHead* head;
   SpRec* rec;
-  float2* first_ml;   // [B * Hq]           pieces that start a row block
+  int* starts;        // [B + 1]            first item of each sequence's own keys (decode_attn_kernel<true>)
+  float2* first_ml;   // [B * Hq]           pieces that start a row block: rows by group, kv head, member, head
   float* first_o;     // [B * Hq][128]
-  float2* rest_ml;    // [CTAs][kSpRows]    pieces that start inside one
+  float2* rest_ml;    // [CTAs][kSpRows]    pieces that start inside one: rows of the block
   float* rest_o;      // [CTAs][kSpRows][128]
   unsigned* err;
 };
@@ -115,6 +122,34 @@ __device__ __forceinline__ float sp_exp2(float x) {
   return y;
 }
 
+// Two fp32 operations in one instruction.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ F2 sp_fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ F2 sp_add2(F2 a, F2 b) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float sp_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // 32 columns of this warp's TMEM lanes into registers that hold floats from
 // the start: nothing may touch them before tmem_ld_wait().
 __device__ __forceinline__ void sp_tmem_ld(uint32_t taddr, float* r) {
@@ -129,6 +164,32 @@ __device__ __forceinline__ void sp_tmem_ld(uint32_t taddr, float* r) {
       : "r"(taddr));
 }
 
+// O of this row times f, 16 columns at a time (the scores stay in registers meanwhile).
+__device__ __forceinline__ void sp_tmem_scale(uint32_t taddr, float f) {
+  uint32_t r[16];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr + (uint32_t)(c * 16)));
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      asm volatile("" : "+r"(r[i]));
+      r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+    }
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};" ::"r"(taddr + (uint32_t)(c * 16)),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+  }
+}
+
 // D[tmem] (+)= A[tmem] * B[smem]: the A operand's rows are TMEM lanes, two bf16 to a column.
 __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
                                               uint32_t accumulate) {
@@ -140,24 +201,52 @@ __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, 
       : "memory");
 }
 
+// The group that sequence b counts in (-1: none): live rows only.  `flag`: report what is out of range.
+__device__ __forceinline__ int sp_group_of(const SharedArgs& a, int b, bool flag = false) {
+  const int g = a.prefix_group[b];
+  const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0, nk = a.cu_k[b + 1] - a.cu_k[b];
+  if (g < -1 || g >= a.groups || (nq >= 1 && (q0 < 0 || q0 >= a.num_q_rows))) {
+    if (flag) raise_error(a.err, ERR_BAD_INDEX);
+    return -1;
+  }
+  return nq < 1 || nk <= 0 ? -1 : g;  // padding rows of a captured batch, rows without keys
+}
+
+// Members and shortest member (keys) of each group.  All `threads` threads of the CTA call it.
+__device__ __forceinline__ void sp_count_groups(const SharedArgs& a, int* cnt, int* least, int threads) {
+  for (int g = threadIdx.x; g < a.groups; g += threads) {
+    cnt[g] = 0;
+    least[g] = 0x7fffffff;
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.B; b += threads) {
+    const int g = sp_group_of(a, b);
+    if (g >= 0) {
+      atomicAdd(&cnt[g], 1);
+      atomicMin(&least[g], a.cu_k[b + 1] - a.cu_k[b]);
+    }
+  }
+  __syncthreads();
+}
+
+// Pages of a group's prefix that count: whole ones that every member sees; a group of one shares none.
+__device__ __forceinline__ int sp_shared_pages(const SharedArgs& a, int given, int members, int least) {
+  return members < 2 ? 0 : min(max(min(given, least), 0) / a.page, a.bt_width);
+}
+
 // Builds the plan (every CTA the same) in shared memory.  All threads call it.
 __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
   const int tid = threadIdx.x, lane = tid & 31;
   for (int g = tid; g < a.groups; g += kSpThreads) {
     s.cnt[g] = 0;
     s.least[g] = 0x7fffffff;
+    s.tiles[g] = a.prefix_len[g];
   }
   __syncthreads();
   for (int b = tid; b < a.B; b += kSpThreads) {
-    int g = a.prefix_group[b];
-    const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0, nk = a.cu_k[b + 1] - a.cu_k[b];
-    if (g < -1 || g >= a.groups || (nq >= 1 && (q0 < 0 || q0 >= a.num_q_rows))) {
-      if (blockIdx.x == 0) raise_error(a.err, ERR_BAD_INDEX);
-      g = -1;
-    }
-    if (nq < 1 || nk <= 0) g = -1;  // padding rows of a captured batch
+    const int g = sp_group_of(a, b, blockIdx.x == 0);
     s.group[b] = (short)g;
-    if (g >= 0) atomicMin(&s.least[g], nk);
+    if (g >= 0) atomicMin(&s.least[g], a.cu_k[b + 1] - a.cu_k[b]);
   }
   __syncthreads();
   if (tid < 32) {
@@ -185,12 +274,7 @@ __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
       long long u = 0;
       if (g < a.groups) {
         n = s.cnt[g];
-        if (n >= 2) {
-          // whole pages that every member sees
-          int keys = min(a.prefix_len[g], s.least[g]);
-          const int pages = min(max(keys, 0) / a.page, a.bt_width);
-          tiles = pages * (a.page / kSpTile);
-        }
+        tiles = sp_shared_pages(a, s.tiles[g], n, s.least[g]) * (a.page / kSpTile);
         u = (long long)((n + a.members - 1) / a.members) * a.Hkv * tiles;
       }
       int ni = n;
@@ -274,8 +358,10 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   uint64_t* s_full = q_full + 2;           // [2]
   uint64_t* p_full = q_full + 4;           // [2]
   uint64_t* o_done = q_full + 6;           // [2]
-  uint64_t* drain = q_full + 8;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 9);
+  uint64_t* p_half = q_full + 8;           // [2] the first 64 keys of P are there
+  uint64_t* drain = q_full + 10;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 11);
+  volatile int* bad = reinterpret_cast<int*>(q_full + 12);  // some page is missing: the softmax looks which
   SpPlan& plan = *reinterpret_cast<SpPlan*>(smem + kSpPlan);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -287,9 +373,11 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       mbar_init(&q_full[t], 4);  // a warp's lane 0 arrives for its rows
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[t], 4);
+      mbar_init(&p_half[t], 4);
       mbar_init(&o_done[t], 1);
     }
     mbar_init(drain, 1);
+    *bad = 0;
     fence_mbar_init();
   }
   griddep_wait();
@@ -312,6 +400,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         r.blocks = (plan.start[g + 1] - plan.start[g] + a.members - 1) / a.members;
         r.rank = plan.rank[b];
         r.off = plan.off[g];
+        r.start = plan.start[g];
+        r.members = plan.start[g + 1] - plan.start[g];
       }
       a.rec[b] = r;
     }
@@ -330,9 +420,10 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   const uint32_t tmem = *tmem_slot;  // S / P of tile t at t * 128, O of tile t at 256 + t * 128
   const uint32_t base = smem_u32(smem);
 
-  if (warp == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSpRegsIssue));
     // ---- producer
-    if (lane == 0) {
+    if (warp == 0 && lane == 0) {
       int it = 0;      // loads issued; load it is in slot it % kSpSlots
       bool ok = true;
       for (long long u = u_beg; ok && u < u_end;) {
@@ -342,6 +433,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           long long row = sp_tile_row(a, leader, k);
           if (row < 0) {
             raise_error(a.err, ERR_BAD_INDEX);
+            *bad = 1;
             row = a.num_slots;  // behind the cache: the load fills zeros (the softmax masks the tile)
           }
 #pragma unroll
@@ -364,9 +456,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       for (int i = it > kSpSlots ? it - kSpSlots : 0; i < it; ++i)
         mbar_wait(&full[i % kSpSlots], (uint32_t)(i / kSpSlots) & 1u, a.err);
     }
-  } else if (warp == 1) {
     // ---- MMA issuer
-    if (lane == 0) {
+    if (warp == 1 && lane == 0) {
       const uint32_t idesc_s = umma_idesc_bf16(128, kSpTile);
       const uint32_t idesc_o = umma_idesc_bf16(128, 128) | (1u << 16);  // B (V) MN-major
       int it = 0, seg[2] = {0, 0}, step[2] = {0, 0};
@@ -383,10 +474,10 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         }
         tc_commit(&s_full[t]);
       };
-      auto values = [&](int t, int i, bool acc) {  // O_t (+)= P_t V, V in load i
+      auto values = [&](int t, int i, int half, bool acc) {  // O_t (+)= P_t V over 64 keys, V in load i
         const uint32_t vb = base + kSpRing + (uint32_t)(i % kSpSlots) * 32768u;
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
+        for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
           tc_mma_f16_ts(tmem + 256u + (uint32_t)t * 128u, tmem + (uint32_t)t * 128u + (uint32_t)kk * 8u,
                         umma_desc_sw128_mn(vb + (uint32_t)kk * 2048u, 16384u), idesc_o, (acc || kk > 0) ? 1u : 0u);
       };
@@ -405,11 +496,15 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           const bool more = k + 1 < g.k1;
           ok = wait_slot(it + 1) && (!more || wait_slot(it + 2));
           for (int t = 0; ok && t < g.nt; ++t) {
+            ok = mbar_wait(&p_half[t], (uint32_t)step[t] & 1u, a.err);
+            if (!ok) break;
+            tc_fence_after();
+            values(t, it + 1, 0, k > g.k0);
             ok = mbar_wait(&p_full[t], (uint32_t)step[t] & 1u, a.err);
             if (!ok) break;
             ++step[t];
             tc_fence_after();
-            values(t, it + 1, k > g.k0);
+            values(t, it + 1, 1, true);
             // S_t's next scores overwrite P_t: MMAs of one thread run in the order of issue
             if (more) scores(t, it + 2);
             else tc_commit(&o_done[t]);
@@ -426,8 +521,9 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       mbar_wait(drain, 0u, a.err);
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSpRegsSoftmax));
     // ---- softmax: one thread per row of its tile
-    const int t = warp >= 6;
+    const int t = warp >= 8;
     const int q4 = warp & 3;             // TMEM lane quarter of this warp
     const int row = q4 * 32 + lane;      // of the tile
     const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
@@ -438,21 +534,26 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       const SpSeg g = sp_segment(a, plan, u, u_end);
       u += g.k1 - g.k0;
       if (t >= g.nt) continue;
-      const int r = t * 128 + row;  // row of the block: member r / G, head r % G
-      const bool valid = r < g.rows;
-      const int m0 = plan.start[g.g] + g.block * a.members;
-      const int b = plan.member[valid ? m0 + r / a.G : m0];
-      const int hq = g.h * a.G + r % a.G;
+      const int m0 = plan.start[g.g] + g.block * a.members;  // first member of the block
+      uint8_t* qrows = smem + kSpQ + t * 32768 + q4 * 4096;  // this warp's 32 rows (64 dims; the others 16 KB on)
       {
-        // the row's 128 dims in the swizzled K-major layout of the MMA (zeros behind the last member)
-        uint8_t* dst = smem + kSpQ + t * 32768 + row * 128;
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)a.cu_q[b] * a.q_stride + hq * 128);
+        // the rows in the swizzled K-major layout of the MMA, two rows of 256 bytes a load
+        const int r = t * 128 + row;  // row of the block: member r / G, head r % G (zeros behind the last member)
+        const int i = r / a.G;
+        const bool valid = r < g.rows;
+        const long long from = valid ? (long long)a.cu_q[plan.member[m0 + i]] * a.q_stride + (g.h * a.G + r - i * a.G) * 128
+                                     : -1;
         uint4 v[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) v[c] = valid ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < 16; ++c) {
+          const long long at = __shfl_sync(0xffffffffu, from, 2 * c + (lane >> 4));
+          v[c] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.q + at) + (lane & 15)) : make_uint4(0u, 0u, 0u, 0u);
+        }
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = v[c];
+        for (int c = 0; c < 16; ++c) {
+          const int rr = 2 * c + (lane >> 4), ch = lane & 15;
+          *reinterpret_cast<uint4*>(qrows + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = v[c];
+        }
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
@@ -472,10 +573,18 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         // every use of s stays behind the wait
 #pragma unroll
         for (int i = 0; i < 128; ++i) asm volatile("" : "+f"(s[i]));
-        const bool there = sp_tile_row(a, leader, k) >= 0;
-        float mt = s[0];
+        const bool there = !*bad || sp_tile_row(a, leader, k) >= 0;
+        float mx[8];
 #pragma unroll
-        for (int i = 1; i < 128; ++i) mt = fmaxf(mt, s[i]);
+        for (int i = 0; i < 8; ++i) mx[i] = sp_max3(s[i], s[i + 8], s[i + 16]);
+#pragma unroll
+        for (int i = 24; i < 120; i += 16) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx[e] = sp_max3(mx[e], s[i + e], s[i + 8 + e]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx[i] = fmaxf(mx[i], s[120 + i]);
+        float mt = fmaxf(sp_max3(sp_max3(mx[0], mx[1], mx[2]), mx[3], mx[4]), sp_max3(mx[5], mx[6], mx[7]));
         mt = there ? mt * a.scale_log2 : -INFINITY;
         if (!there) {
 #pragma unroll
@@ -485,39 +594,32 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         if (__any_sync(0xffffffffu, mt > m + kSpLazy)) {
           const float m_new = fmaxf(m, mt);
           const float alpha = m == -INFINITY ? 0.f : sp_exp2(m - m_new);
-          if (k > g.k0) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t x[32];
-              tmem_ld_32x32b_x32(to + (uint32_t)(c * 32), x);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
-              tmem_st_32x32b_x32(to + (uint32_t)(c * 32), x);
-            }
-          }
+          if (k > g.k0) sp_tmem_scale(to, alpha);
           l *= alpha;
           m = m_new;
         }
         const float mm = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: P = 0
-        float rs = 0.f;
+        const F2 scale2 = {a.scale_log2, a.scale_log2}, minus = {-mm, -mm};
+        F2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pk[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float p0 = sp_exp2(fmaf(s[c * 64 + 2 * i], a.scale_log2, -mm));
-            const float p1 = sp_exp2(fmaf(s[c * 64 + 2 * i + 1], a.scale_log2, -mm));
-            rs += p0 + p1;
-            pk[i] = pack_bf16x2(p0, p1);
+            const F2 y = sp_fma2({s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]}, scale2, minus);
+            const F2 e = {sp_exp2(y.x), sp_exp2(y.y)};
+            sum[i & 3] = sp_add2(sum[i & 3], e);
+            pk[i] = pack_bf16x2(e.x, e.y);
           }
           tmem_st_32x32b_x32(ts + (uint32_t)(c * 32), pk);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          // the PV product of the first 64 keys runs while the others are exponentiated
+          if (lane == 0) mbar_arrive(c ? &p_full[t] : &p_half[t]);
         }
-        l += rs;
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        const F2 rs = sp_add2(sp_add2(sum[0], sum[1]), sp_add2(sum[2], sum[3]));
+        l += rs.x + rs.y;
       }
       if (!ok) break;
       // ---- the segment's partial
@@ -527,21 +629,34 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       ++seg;
       tc_fence_after();
       const bool first = g.k0 == 0;
-      const size_t at = first ? (size_t)b * a.Hq + hq : (size_t)blockIdx.x * kSpRows + r;
-      float* po = (first ? a.first_o : a.rest_o) + at * 128;
-      if (valid) (first ? a.first_ml : a.rest_ml)[at] = make_float2(m, l);
+      const size_t at = first ? ((size_t)plan.start[g.g] * a.Hkv +
+                                 (size_t)g.h * (plan.start[g.g + 1] - plan.start[g.g]) + g.block * a.members) * a.G
+                              : (size_t)blockIdx.x * kSpRows;
+      const int r0 = t * 128 + q4 * 32;  // this warp's first row of the block
+      if (r0 + lane < g.rows) (first ? a.first_ml : a.rest_ml)[at + r0 + lane] = make_float2(m, l);
+      float* po = (first ? a.first_o : a.rest_o) + (at + r0) * 128;
+      // 32 columns at a time through this warp's part of the Q tile (its MMAs
+      // are done), so that a store writes whole 128-byte lines
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        uint32_t x[32];
-        tmem_ld_32x32b_x32(to + (uint32_t)(c * 32), x);
+        float x[32];
+        sp_tmem_ld(to + (uint32_t)(c * 32), x);
         tmem_ld_wait();
-        if (valid) {
+        uint8_t* stage = qrows + (c & 1) * 16384;
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(po + c * 32 + i) =
-                make_float4(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]),
-                            __uint_as_float(x[i + 3]));
+        for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(x[i]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+              make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = 4 * i + (lane >> 3);
+          const float4 y = *reinterpret_cast<const float4*>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+          if (r0 + rr < g.rows) *reinterpret_cast<float4*>(po + rr * 128 + c * 32 + (lane & 7) * 4) = y;
         }
+        __syncwarp();
       }
     }
   }

@@ -72,7 +72,7 @@ _SIGNATURES = {
                                     ctypes.c_ulonglong, ctypes.c_ulonglong, _c_void_p, _c_void_p], _i),
     "b200_select_tokens_exchange": ([_c_void_p, _i, _i, _i, _c_void_p, _c_void_p, _c_void_p, _ll,
                                      _c_void_p, _c_void_p], _i),
-    "b200_shared_prefix_workspace_bytes": ([_i, _i, _i, ctypes.POINTER(_sz)], _i),
+    "b200_shared_prefix_workspace_bytes": ([_i, _i, _i, _i, ctypes.POINTER(_sz)], _i),
     "b200_shared_prefix_attention": ([_c_void_p, _ll, _i, _c_void_p, _c_void_p, _ll, _c_void_p, _i, _i,
                                       _c_void_p, _c_void_p, _i, _i, _i, _i, _i, _f, _c_void_p,
                                       _c_void_p, _i, _c_void_p, _ll, _c_void_p, _sz, _c_void_p], _i),
@@ -605,17 +605,17 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | N
     return out
 
 
-_prefix_ws_bytes: dict[tuple[int, int, int, int], int] = {}
+_prefix_ws_bytes: dict[tuple[int, ...], int] = {}
 
 
-def shared_prefix_workspace_bytes(max_seqs: int, max_seqlen_k: int, num_heads: int) -> int:
+def shared_prefix_workspace_bytes(max_seqs: int, max_seqlen_k: int, num_heads: int, num_kv_heads: int) -> int:
     """(of the current device: its size depends on the SM count)"""
-    key = (torch.cuda.current_device(), max_seqs, max_seqlen_k, num_heads)
+    key = (torch.cuda.current_device(), max_seqs, max_seqlen_k, num_heads, num_kv_heads)
     n = _prefix_ws_bytes.get(key)
     if n is None:
         size = ctypes.c_size_t(0)
         _check(load_library().b200_shared_prefix_workspace_bytes(max_seqs, max_seqlen_k, num_heads,
-                                                                 ctypes.byref(size)),
+                                                                 num_kv_heads, ctypes.byref(size)),
                "b200_shared_prefix_workspace_bytes")
         if len(_prefix_ws_bytes) > 4096:
             _prefix_ws_bytes.clear()
@@ -655,7 +655,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         elif out.shape != q.shape or out.stride(-1) != 1 or out.stride(1) != 128:
             raise ValueError(f"out must be {tuple(q.shape)} with contiguous heads")
         pages, page, Hkv, _ = k_cache.shape
-        ws = workspace("shared_prefix", shared_prefix_workspace_bytes(B, int(max_seqlen_k), Hq), q.device)
+        ws = workspace("shared_prefix", shared_prefix_workspace_bytes(B, int(max_seqlen_k), Hq, Hkv), q.device)
         _check(load_library().b200_shared_prefix_attention(
             q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), pages * page,
             block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cu_seqlens_q.data_ptr(),
