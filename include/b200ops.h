@@ -307,8 +307,8 @@ int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, i
  *  - B <= 1024, num_groups <= 1024, Hq / Hkv <= 8, page a multiple of 256,
  *    softmax_scale > 0.
  *  - workspace: b200_shared_prefix_workspace_bytes(B, max_seqlen_k, Hq, Hkv) bytes,
- *    256-byte aligned, its first 256 KiB + 256 bytes zero before the first
- *    call (they are zero again after every call).  Calls that share a
+ *    256-byte aligned, its first 256 bytes zero before the first call (they
+ *    are zero again after every call).  Calls that share a
  *    workspace must not overlap on the GPU, and it is not the workspace of
  *    b200_paged_attention. */
 int b200_shared_prefix_attention(const void* q, long long q_stride, int num_q_rows, const void* k_cache,

@@ -23,6 +23,7 @@
 #include "exchange.cuh"
 #include "metadata.cuh"
 #include "pages.cuh"
+#include "own_keys.cuh"
 #include "prefill_tc.cuh"
 #include "shared_prefix.cuh"
 #include "gemm.cuh"
@@ -314,7 +315,7 @@ int launch_decode(DeviceState* ds, const CUtensorMap& tmK, const CUtensorMap& tm
   attr[0].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_attn_kernel<false>, tmK, tmV, tmQ, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_attn_kernel, tmK, tmV, tmQ, a);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "decode attention launch: %s", cudaGetErrorString(e));
   return B200_OK;
 }
@@ -1293,7 +1294,7 @@ int b200_paged_attention(const void* q, long long q_stride, int num_q_rows, cons
     a.out = static_cast<__nv_bfloat16*>(out); a.out_stride = out_stride;
     a.err = ds->err;
     const int smem = dec_smem_bytes();
-    if (int r = ensure_smem(ds, 2u, decode_attn_kernel<false>, smem)) return r;
+    if (int r = ensure_smem(ds, 2u, decode_attn_kernel, smem)) return r;
     if (int r = launch_decode(ds, tmK, tmV, tmQ, a, smem, st)) return r;
     return check_launch("decode_attn_kernel");
   }
@@ -1528,13 +1529,13 @@ extern "C" int b200_paged_decode_attention_static(
   a.out = static_cast<__nv_bfloat16*>(out); a.out_stride = out_stride;
   a.err = ds->err;
   const int smem = dec_smem_bytes();
-  if (int r = ensure_smem(ds, 2u, decode_attn_kernel<false>, smem)) return r;
+  if (int r = ensure_smem(ds, 2u, decode_attn_kernel, smem)) return r;
   if (int r = launch_decode(ds, tmK, tmV, tmQ, a, smem, st)) return r;
   return check_launch("decode_attn_kernel");
 }
 
 // ===========================================================================
-// Decode attention with shared prefixes (shared_prefix.cuh, decode_attention.cuh)
+// Decode attention with shared prefixes (shared_prefix.cuh, own_keys.cuh)
 // ===========================================================================
 namespace {
 
@@ -1543,11 +1544,11 @@ size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 // Items (of the sequences' own keys) the workspace has room for: 512 keys each
 // and one more per sequence, or as many short ones as there are warps.
 long long shared_items(int num_sms, int seqs, int max_seqlen_k, int Hkv) {
-  return (long long)seqs * ((max_seqlen_k + kDecItem - 1) / kDecItem + 1) +
-         ((long long)num_sms * kDecWarps + Hkv - 1) / Hkv;
+  return (long long)seqs * ((max_seqlen_k + kOwnItem - 1) / kOwnItem + 1) +
+         ((long long)num_sms * kOwnWarps + Hkv - 1) / Hkv;
 }
 
-// The workspace: the decode kernel's head and items, the sequences' records
+// The workspace: the queue, the parts of the own keys, the sequences' records
 // and first items, the partials of the pieces that start a row block, those of
 // the others.
 struct SharedLayout {
@@ -1557,20 +1558,20 @@ SharedLayout shared_layout(int num_sms, int seqs, int max_seqlen_k, int Hq, int 
   const size_t items = (size_t)shared_items(num_sms, seqs, max_seqlen_k, Hkv), rows = (size_t)seqs * Hq,
                rest = (size_t)num_sms * kSpRows;
   SharedLayout l{};
-  size_t at = align256(kDecSchedBytes);
+  size_t at = kOwnQueueBytes;
   auto take = [&](size_t bytes) {
     const size_t from = at;
     at += align256(bytes);
     return from;
   };
-  l.part_o = take(items * Hq * kDecHD * sizeof(float));
+  l.part_o = take(items * Hq * kOwnHD * sizeof(float));
   l.part_ml = take(items * Hq * sizeof(float2));
   l.head = take(kSpRecBytes);
   l.starts = take((kSpMaxSeqs + 1) * sizeof(int));
   l.first_ml = take(rows * sizeof(float2));
-  l.first_o = take(rows * kDecHD * sizeof(float));
+  l.first_o = take(rows * kOwnHD * sizeof(float));
   l.rest_ml = take(rest * sizeof(float2));
-  l.rest_o = take(rest * kDecHD * sizeof(float));
+  l.rest_o = take(rest * kOwnHD * sizeof(float));
   l.total = at;
   return l;
 }
@@ -1637,56 +1638,48 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int G = Hq / Hkv;
   CUtensorMap tmK, tmV, tmQ;
-  const uint64_t row = (uint64_t)Hkv * kDecHD * 2;
-  DecodeArgs a{};
-  a.block_tables = block_tables; a.bt_stride = bt_stride; a.bt_width = bt_width;
-  a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k;
-  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = G; a.page = page; a.q_box_rows = Hq < 8 ? Hq : 8;
-  a.num_slots = num_slots;
-  a.scale_log2 = softmax_scale * 1.4426950408889634f;
-  a.out = static_cast<__nv_bfloat16*>(out); a.out_stride = out_stride;
-  a.err = ds->err;
+  const uint64_t row = (uint64_t)Hkv * kOwnHD * 2;
   char* ws = static_cast<char*>(workspace);
-  a.sched = static_cast<int*>(workspace);
-  a.cap_items = shared_items(ds->num_sms, B, max_seqlen_k, Hkv);
-  a.part_o = reinterpret_cast<float*>(ws + l.part_o);
-  a.part_ml = reinterpret_cast<float*>(ws + l.part_ml);
-  SharedArgs& s = a.sp;
+  SharedArgs s{};
   s.q = static_cast<const __nv_bfloat16*>(q); s.q_stride = q_stride; s.num_q_rows = num_q_rows;
   s.cu_q = cu_seqlens_q; s.cu_k = cu_seqlens_k;
   s.block_tables = block_tables; s.bt_stride = bt_stride; s.bt_width = bt_width;
   s.prefix_group = prefix_group; s.prefix_len = prefix_len; s.groups = num_groups;
   s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.G = G; s.page = page; s.members = kSpRows / G;
-  s.num_slots = num_slots; s.scale_log2 = a.scale_log2;
+  s.num_slots = num_slots; s.scale_log2 = softmax_scale * 1.4426950408889634f;
   s.head = reinterpret_cast<SpHead*>(ws + l.head);
   s.rec = reinterpret_cast<SpRec*>(ws + l.head + sizeof(SpHead));
+  s.queue = static_cast<int*>(workspace);
   s.starts = reinterpret_cast<int*>(ws + l.starts);
+  s.cap_items = shared_items(ds->num_sms, B, max_seqlen_k, Hkv);
+  s.part_o = reinterpret_cast<float*>(ws + l.part_o);
+  s.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
+  s.out = static_cast<__nv_bfloat16*>(out); s.out_stride = out_stride;
   s.first_ml = reinterpret_cast<float2*>(ws + l.first_ml);
   s.first_o = reinterpret_cast<float*>(ws + l.first_o);
   s.rest_ml = reinterpret_cast<float2*>(ws + l.rest_ml);
   s.rest_o = reinterpret_cast<float*>(ws + l.rest_o);
   s.err = ds->err;
   // the shared part
-  if (int r = make_tmap_3d(&tmK, k_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kSpTile)) return r;
-  if (int r = make_tmap_3d(&tmV, v_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kSpTile)) return r;
+  if (int r = make_tmap_3d(&tmK, k_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kSpTile)) return r;
+  if (int r = make_tmap_3d(&tmV, v_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kSpTile)) return r;
   if (int r = ensure_smem(ds, 32u, shared_prefix_kernel, kSpSmemBytes)) return r;
   cudaError_t e = launch_ex(shared_prefix_kernel, dim3(ds->num_sms), dim3(kSpThreads), kSpSmemBytes, st, nullptr, 0,
                             tmK, tmV, s);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
   if (int r = check_launch("shared_prefix_kernel")) return r;
   // every sequence's own keys
-  if (int r = make_tmap_3d(&tmK, k_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kDecTile)) return r;
-  if (int r = make_tmap_3d(&tmV, v_cache, kDecHD, Hkv, (uint64_t)num_slots, kDecHD * 2, row, 64, 1, kDecTile)) return r;
-  if (int r = make_tmap_3d(&tmQ, q, kDecHD, Hq, (uint64_t)num_q_rows, kDecHD * 2, (uint64_t)q_stride * 2, 64,
-                           (uint32_t)a.q_box_rows, 1))
+  if (int r = make_tmap_3d(&tmK, k_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kOwnTile)) return r;
+  if (int r = make_tmap_3d(&tmV, v_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kOwnTile)) return r;
+  if (int r = make_tmap_3d(&tmQ, q, kOwnHD, Hq, (uint64_t)num_q_rows, kOwnHD * 2, (uint64_t)q_stride * 2, 64,
+                           (uint32_t)std::min(Hq, 8), 1))
     return r;
-  const int smem = dec_smem_bytes<true>();
-  if (int r = ensure_smem(ds, 64u, decode_attn_kernel<true>, smem)) return r;
-  e = launch_overlapped(decode_attn_kernel<true>, ds->num_sms, kDecWarps * 32, smem, st, tmK, tmV, tmQ, a);
+  if (int r = ensure_smem(ds, 64u, own_keys_kernel, kOwnSmemBytes)) return r;
+  e = launch_overlapped(own_keys_kernel, ds->num_sms, kOwnThreads, kOwnSmemBytes, st, tmK, tmV, tmQ, s);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
-  if (int r = check_launch("decode_attn_kernel(shared prefix)")) return r;
+  if (int r = check_launch("own_keys_kernel")) return r;
   // the parts of each row
-  e = launch_overlapped(shared_merge_kernel, (B * Hq + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, st, a);
+  e = launch_overlapped(shared_merge_kernel, (B * Hq + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, st, s);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
   return check_launch("shared_merge_kernel");
 }

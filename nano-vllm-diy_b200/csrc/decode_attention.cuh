@@ -30,15 +30,8 @@
 // The launch shape depends only on the SM count; context lengths are read
 // from cu_seqlens_k on the device (CUDA-graph safe; rows with q length <= 0
 // are graph padding and are skipped).
-//
-// decode_attn_kernel<true> is the part of attention with shared prefixes
-// (shared_prefix.cuh) that streams every sequence's own keys: items start
-// behind the prefix, every part of a row that has several is left as a partial,
-// and shared_merge_kernel puts the parts together.  No warp waits on another
-// one, so the launch is an ordinary one, which may overlap the prefix kernel.
 #pragma once
 #include "common.cuh"
-#include "shared_prefix.cuh"
 
 namespace b200 {
 
@@ -46,7 +39,6 @@ constexpr int kDecHD = 128;
 constexpr int kDecItem = 512;        // tokens per work item (may span pages); sizes the workspace
 constexpr int kDecItemLong = 1024;   // tokens per item when the batch's mean context is long
 constexpr int kDecLongMean = 2048;   // mean context (keys per sequence) from which items are long
-constexpr int kDecItemLeast = 64;    // with shared prefixes, when there are few keys
 constexpr int kDecItemPages = 4;     // block-table entries an item can touch (pages >= 256 tokens)
 constexpr int kDecTile = 32;      // tokens per pipeline stage
 constexpr int kDecStages = 3;
@@ -79,7 +71,6 @@ struct DecodeArgs {
   __nv_bfloat16* out;
   long long out_stride;
   unsigned* err;
-  SharedArgs sp;         // decode_attn_kernel<true> only
 };
 
 struct DecTile {
@@ -103,11 +94,9 @@ __device__ __forceinline__ int ld_acquire_gpu_s32(const int* p) {
   return v;
 }
 
-template <bool kShared = false>
 __host__ __device__ constexpr int dec_smem_bytes() {
   return 1024 + kDecWarps * kDecWarpBytes + kDecWarps * kDecStages * 8 +
-         kDecWarps * kDecStages * (int)sizeof(DecTile) +
-         (8 + (kShared ? 2 : 1) * kDecMaxSeqs + 1) * (int)sizeof(int);
+         kDecWarps * kDecStages * (int)sizeof(DecTile) + (8 + kDecMaxSeqs + 1) * (int)sizeof(int);
 }
 
 // byte offset of 16-byte chunk `ch` (0..15 over 128 dims) of row `r` in a
@@ -116,7 +105,6 @@ __device__ __forceinline__ uint32_t tswz(int half_bytes, int r, int ch) {
   return (uint32_t)((ch >> 3) * half_bytes + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
 }
 
-template <bool kShared>
 __global__ void __launch_bounds__(128, 1)
     decode_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                        const __grid_constant__ CUtensorMap tmQ, const DecodeArgs a) {
@@ -131,7 +119,6 @@ __global__ void __launch_bounds__(128, 1)
   int* s_scan = reinterpret_cast<int*>(smem + kDecWarps * kDecWarpBytes + kDecWarps * kDecStages * 8 +
                                        kDecWarps * kDecStages * sizeof(DecTile));
   int* s_start = s_scan + 8;
-  int* s_prefix = s_start + kDecMaxSeqs + 1;  // kShared: keys of the shared prefix
   int* sched = a.sched;
   int* unit_done = a.sched + 64;  // [b * Hkv + h]: items of the unit published
 
@@ -146,22 +133,8 @@ __global__ void __launch_bounds__(128, 1)
   }
   // the barrier setup above overlaps the previous kernel's tail
   // (programmatic dependent launch); sequence lengths, Q and the cache below
-  if constexpr (kShared) {
-    // The inputs are older than the prefix kernel, which waited for them; its
-    // own results are left to the merge.
-    int* cnt = reinterpret_cast<int*>(smem);  // in the rings, before their first load
-    int* least = cnt + kSpMaxGroups;
-    sp_count_groups(a.sp, cnt, least, blockDim.x);
-    for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
-      const int g = sp_group_of(a.sp, b);
-      s_prefix[b] = g >= 0 ? sp_shared_pages(a.sp, a.sp.prefix_len[g], cnt[g], least[g]) * a.page : 0;
-    }
-    fence_proxy_async_smem();
-    __syncthreads();
-  } else {
-    griddep_wait();
-    griddep_launch_dependents();
-  }
+  griddep_wait();
+  griddep_launch_dependents();
 
   // ---- plan: exclusive prefix sum of items per sequence (identical in every
   // CTA).  Item length: 512 keys, or 1024 when the batch's mean context is at
@@ -176,7 +149,7 @@ __global__ void __launch_bounds__(128, 1)
     int active = 0;
     for (int b = beg; b < end; ++b) {
       const int nq = a.cu_q[b + 1] - a.cu_q[b];
-      const int nk = a.cu_k[b + 1] - a.cu_k[b] - (kShared ? s_prefix[b] : 0);
+      const int nk = a.cu_k[b + 1] - a.cu_k[b];
       if (nq >= 1 && nk > 0) {
         keys += nk;
         ++active;
@@ -200,16 +173,11 @@ __global__ void __launch_bounds__(128, 1)
       all_active += s_scan[w];
     }
     if (all_active > 0 && all_keys >= (long long)kDecLongMean * all_active) item_len = kDecItemLong;
-    if constexpr (kShared) {
-      // a short batch: items small enough for every warp to have one
-      const long long each = (all_keys * a.Hkv + gridDim.x * kDecWarps - 1) / (gridDim.x * kDecWarps);
-      if (each < kDecItem) item_len = max(kDecItemLeast, (int)(each + kDecTile - 1) / kDecTile * kDecTile);
-    }
     __syncthreads();  // s_scan is reused by the scan below
     int local = 0;
     for (int b = beg; b < end; ++b) {
       const int nq = a.cu_q[b + 1] - a.cu_q[b];
-      const int nk = a.cu_k[b + 1] - a.cu_k[b] - (kShared ? s_prefix[b] : 0);
+      const int nk = a.cu_k[b + 1] - a.cu_k[b];
       const int cnt = (nq >= 1 && nk > 0) ? (nk + item_len - 1) / item_len : 0;
       s_start[b] = cnt;
       local += cnt;
@@ -233,13 +201,8 @@ __global__ void __launch_bounds__(128, 1)
     __syncthreads();
   }
   const int total_chunks = s_start[a.B];
-  if constexpr (kShared) {
-    if (blockIdx.x == 0)
-      for (int b = threadIdx.x; b <= a.B; b += blockDim.x) a.sp.starts[b] = s_start[b];
-  }
   if ((long long)total_chunks > a.cap_items) {
     if (blockIdx.x == 0 && threadIdx.x == 0) raise_error(a.err, ERR_BAD_INDEX);
-    if constexpr (kShared) griddep_wait();
     return;
   }
   const int items = total_chunks * a.Hkv;
@@ -272,8 +235,7 @@ __global__ void __launch_bounds__(128, 1)
       if (s_start[mid] <= c) lo = mid; else hi = mid - 1;
     }
     const int b = lo;
-    const int shared = kShared ? s_prefix[b] : 0;
-    const int j0 = shared + (c - s_start[b]) * item_len;
+    const int j0 = (c - s_start[b]) * item_len;
     const int nk = a.cu_k[b + 1] - a.cu_k[b];
     const int ntok_item = min(item_len, nk - j0);
     // the block-table entries of the item's pages (one per lane 0..3)
@@ -286,7 +248,7 @@ __global__ void __launch_bounds__(128, 1)
     blk2 = __shfl_sync(0xffffffffu, e, 2);
     blk3 = __shfl_sync(0xffffffffu, e, 3);
     cur.b = b; cur.h = h; cur.c = c;
-    cur.npages = s_start[b + 1] - s_start[b] + (shared > 0);  // > 1: parts to merge
+    cur.npages = s_start[b + 1] - s_start[b];
     cur.qrow = a.cu_q[b];
     cur.ntok = ntok_item;
     cur.j0 = j0;
@@ -515,7 +477,7 @@ __global__ void __launch_bounds__(128, 1)
           *reinterpret_cast<float2*>(a.part_ml + ((size_t)d.c * a.Hq + hq) * 2) = make_float2(m_run[e], l_run[e]);
       }
     }
-    if constexpr (!kShared) pending_unit = d.b * a.Hkv + d.h;
+    pending_unit = d.b * a.Hkv + d.h;
   }
   publish_pending();
   // drain: every issued tile has landed before the CTA's shared memory is released
@@ -524,11 +486,6 @@ __global__ void __launch_bounds__(128, 1)
       mbar_wait(&s_bar[t % kDecStages], (uint32_t)(t / kDecStages) & 1u, a.err);
   }
   __syncwarp();
-  if constexpr (kShared) {
-    griddep_launch_dependents();
-    griddep_wait();  // so that this grid's end is the prefix kernel's too
-    return;
-  }
 
   // ---- merge phase: (sequence, kv head) units of sequences split into
   // several items, from a second queue in sequence order.  Each lane owns 4
@@ -614,77 +571,6 @@ __global__ void __launch_bounds__(128, 1)
     atomicExch(&sched[3], 0);
     atomicExch(&sched[4], 0);
   }
-}
-
-// ---------------------------------------------------------------------------
-// The parts of a row of attention with shared prefixes: the prefix's pieces,
-// then the items of the sequence's own keys, always in that order.  One warp
-// per (sequence, query head), 4 dims a lane, four parts in flight: the parts
-// come from L2, so it is latency that counts, and there is a warp for every row.
-// ---------------------------------------------------------------------------
-constexpr int kMergeWarps = 8;
-
-__global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(const DecodeArgs a) {
-  griddep_wait();
-  griddep_launch_dependents();
-  const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= a.B * a.Hq) return;
-  const int b = row / a.Hq, hq = row - b * a.Hq, h = hq / a.G;
-  const SharedArgs& sp = a.sp;
-  const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0;
-  const int c0 = sp.starts[b], own = sp.starts[b + 1] - c0;
-  const SpRec rc = sp.rec[b];
-  if (nq < 1 || (own == 1 && rc.keys == 0)) return;  // padding; written by its one item
-  int p0 = 0, pieces = 0;  // pieces of the prefix: the one that starts the row block, then CTAs p0 ..
-  if (rc.keys > 0) {
-    const long long u0 = rc.off + (long long)(h * rc.blocks + rc.rank / sp.members) * rc.tiles;
-    int end;
-    sp_pieces_inside(sp.head->units, sp.head->pieces, u0, rc.tiles, p0, end);
-    pieces = 1 + end - p0;
-  }
-  const size_t first = ((size_t)rc.start * a.Hkv + (size_t)h * rc.members + rc.rank) * a.G + (hq - h * a.G);
-  const size_t in_block = (size_t)(rc.rank % sp.members) * a.G + (hq - h * a.G);
-  const int n = pieces + own;
-  float M = -INFINITY, L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n; i0 += 4) {
-    float2 ml[4];
-    float4 o[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u;
-      const float2* pm;
-      const float* po;
-      if (i < pieces) {
-        const size_t at = i == 0 ? first : (size_t)(p0 + i - 1) * kSpRows + in_block;
-        pm = (i == 0 ? sp.first_ml : sp.rest_ml) + at;
-        po = (i == 0 ? sp.first_o : sp.rest_o) + at * kDecHD;
-      } else {
-        const size_t at = (size_t)(c0 + i - pieces) * a.Hq + hq;
-        pm = reinterpret_cast<const float2*>(a.part_ml) + at;
-        po = a.part_o + at * kDecHD;
-      }
-      ml[u] = i < n ? __ldcg(pm) : make_float2(-INFINITY, 0.f);
-      o[u] = i < n ? __ldcg(reinterpret_cast<const float4*>(po) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (ml[u].y == 0.f) continue;  // no key there, or none of a finite score
-      const float mn = fmaxf(M, ml[u].x);
-      const float s = fast_exp2(M - mn), w = fast_exp2(ml[u].x - mn);
-      L = L * s + w * ml[u].y;
-      acc.x = acc.x * s + w * o[u].x;
-      acc.y = acc.y * s + w * o[u].y;
-      acc.z = acc.z * s + w * o[u].z;
-      acc.w = acc.w * s + w * o[u].w;
-      M = mn;
-    }
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  uint2 packed;
-  packed.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-  packed.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(a.out + (size_t)q0 * a.out_stride + (size_t)hq * kDecHD + lane * 4) = packed;
 }
 
 }  // namespace b200

@@ -97,7 +97,14 @@ struct SharedArgs {
   float scale_log2;
   SpHead* head;
   SpRec* rec;
-  int* starts;        // [B + 1]            first item of each sequence's own keys (decode_attn_kernel<true>)
+  // own keys (own_keys.cuh)
+  int* queue;         // kOwnQueueBytes, zero between calls
+  int* starts;        // [B + 1]            first item of each sequence
+  float2* part_ml;    // [items][Hq]
+  float* part_o;      // [items][Hq][128]
+  long long cap_items;
+  __nv_bfloat16* out;
+  long long out_stride;
   float2* first_ml;   // [B * Hq]           pieces that start a row block: rows by group, kv head, member, head
   float* first_o;     // [B * Hq][128]
   float2* rest_ml;    // [CTAs][kSpRows]    pieces that start inside one: rows of the block

@@ -226,6 +226,8 @@ def launch_count() -> int:
 _TIMEOUT_BITS = 0x1 | 0x2
 # the GEMM workspace starts with 4 KiB of split-K flags and counters
 _GEMM_FLAG_BYTES = 4096
+# the shared-prefix workspace starts with the queue of its own-keys kernel
+_QUEUE_BYTES = 256
 
 
 def device_error(clear: bool = True) -> int:
@@ -237,8 +239,8 @@ def device_error(clear: bool = True) -> int:
     _check(load_library().b200_device_error(ctypes.byref(v), int(clear)), "b200_device_error")
     if clear and v.value & _TIMEOUT_BITS:
         dev = torch.cuda.current_device()
-        head = attention_workspace_bytes(0, 0, 1)
-        heads = {"attn": head, "shared_prefix": head, "gemm": _GEMM_FLAG_BYTES}
+        heads = {"attn": attention_workspace_bytes(0, 0, 1), "gemm": _GEMM_FLAG_BYTES,
+                 "shared_prefix": _QUEUE_BYTES}
         for (d, kind), buf in _workspaces.items():
             if d == dev and kind in heads:
                 buf[:heads[kind]].zero_()
