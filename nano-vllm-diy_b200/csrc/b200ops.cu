@@ -1552,7 +1552,7 @@ long long shared_items(int num_sms, int seqs, int max_seqlen_k, int Hkv) {
 // and first items, the partials of the pieces that start a row block, those of
 // the others.
 struct SharedLayout {
-  size_t part_o, part_ml, head, starts, first_ml, first_o, rest_ml, rest_o, total;
+  size_t part_o, part_ml, rec, starts, first_ml, first_o, rest_ml, rest_o, total;
 };
 SharedLayout shared_layout(int num_sms, int seqs, int max_seqlen_k, int Hq, int Hkv) {
   const size_t items = (size_t)shared_items(num_sms, seqs, max_seqlen_k, Hkv), rows = (size_t)seqs * Hq,
@@ -1566,7 +1566,7 @@ SharedLayout shared_layout(int num_sms, int seqs, int max_seqlen_k, int Hq, int 
   };
   l.part_o = take(items * Hq * kOwnHD * sizeof(float));
   l.part_ml = take(items * Hq * sizeof(float2));
-  l.head = take(kSpRecBytes);
+  l.rec = take(kSpRecBytes);
   l.starts = take((kSpMaxSeqs + 1) * sizeof(int));
   l.first_ml = take(rows * sizeof(float2));
   l.first_o = take(rows * kOwnHD * sizeof(float));
@@ -1647,8 +1647,7 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   s.prefix_group = prefix_group; s.prefix_len = prefix_len; s.groups = num_groups;
   s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.G = G; s.page = page; s.members = kSpRows / G;
   s.num_slots = num_slots; s.scale_log2 = softmax_scale * 1.4426950408889634f;
-  s.head = reinterpret_cast<SpHead*>(ws + l.head);
-  s.rec = reinterpret_cast<SpRec*>(ws + l.head + sizeof(SpHead));
+  s.rec = reinterpret_cast<SpRec*>(ws + l.rec);
   s.queue = static_cast<int*>(workspace);
   s.starts = reinterpret_cast<int*>(ws + l.starts);
   s.cap_items = shared_items(ds->num_sms, B, max_seqlen_k, Hkv);

@@ -407,13 +407,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(const Sh
   const int c0 = a.starts[b], own = a.starts[b + 1] - c0;
   const SpRec rc = a.rec[b];
   if (nq < 1 || (own == 1 && rc.keys == 0)) return;  // padding; written by its one item
-  int p0 = 0, pieces = 0;  // pieces of the prefix: the one that starts the row block, then CTAs p0 ..
-  if (rc.keys > 0) {
-    const long long u0 = rc.off + (long long)(h * rc.blocks + rc.rank / a.members) * rc.tiles;
-    int end;
-    sp_pieces_inside(a.head->units, a.head->pieces, u0, rc.tiles, p0, end);
-    pieces = 1 + end - p0;
-  }
+  const int pieces = rc.keys > 0 ? rc.split : 0;  // of the prefix: the first, then those of the next jobs
+  const int job = rc.off + (h * rc.blocks + rc.rank / a.members) * rc.split;
   const size_t first = ((size_t)rc.start * a.Hkv + (size_t)h * rc.members + rc.rank) * a.G + (hq - h * a.G);
   const size_t in_block = (size_t)(rc.rank % a.members) * a.G + (hq - h * a.G);
   const int n = pieces + own;
@@ -428,7 +423,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(const Sh
       const float2* pm;
       const float* po;
       if (i < pieces) {
-        const size_t at = i == 0 ? first : (size_t)(p0 + i - 1) * kSpRows + in_block;
+        const size_t at = i == 0 ? first : (size_t)(job + i) * kSpRows + in_block;
         pm = (i == 0 ? a.first_ml : a.rest_ml) + at;
         po = (i == 0 ? a.first_o : a.rest_o) + at * kOwnHD;
       } else {

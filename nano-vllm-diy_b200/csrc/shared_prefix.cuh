@@ -10,14 +10,15 @@
 // keys on the tensor cores, each K / V byte read once for up to 256 rows --,
 // decode_attn_kernel<true> then streams every sequence's own keys and merges.
 //
-// Work: a unit is one 128-key tile of one row block (256 / G members of a group
-// x the G = Hq / Hkv heads of one kv head, at most 256 rows).  The units of all
-// groups, heads and blocks lie on one line that is cut into equal pieces, one
-// per CTA (one CTA per SM): no tail, whatever the groups are.  A piece that
-// starts inside a row block leaves its partial in the CTA's own slot, the
-// piece that starts the block in the rows of the sequences themselves: no
-// place is written twice, and the merge finds the pieces from the same
-// arithmetic, in a fixed order.
+// Work: a row block is up to 256 rows of one group and kv head (256 / G members x
+// the G = Hq / Hkv heads) and its prefix in tiles of 128 keys.  A job is a row
+// block's whole prefix, or one of the equal pieces it is cut into so that no
+// SM idles: a CTA (one on each SM) does one job as long as there are no more
+// jobs than SMs.  How long the pieces are is weighed against the own keys,
+// whose kernel runs on the SMs that get no job (sp_choose_piece).  The piece
+// that starts a row block leaves its partial in the rows of the sequences, the
+// others in a slot of their job: no place is written twice, and the merge finds
+// them by the same arithmetic, in a fixed order.
 //
 // Roles (three warpgroups): warp 0 loads K and V tiles by TMA (a ring of 32 KB
 // slots), warp 1 issues the MMAs (warps 2 and 3 only complete their
@@ -56,8 +57,10 @@ constexpr int kSpPlan = kSpBar + 256;
 
 // The groups of a call, in shared memory.
 struct SpPlan {
-  long long off[kSpMaxGroups + 1];  // first unit of each group
+  unsigned long long keys;          // of all live sequences
+  int off[kSpMaxGroups + 1];        // first job of each group
   int start[kSpMaxGroups + 1];      // first member
+  int split[kSpMaxGroups];          // pieces of a row block
   int cnt[kSpMaxGroups];
   int least[kSpMaxGroups];          // shortest member (keys)
   int tiles[kSpMaxGroups];          // 128-key tiles of the prefix (0: nothing shared)
@@ -68,18 +71,14 @@ struct SpPlan {
 constexpr int kSpSmemBytes = 1024 + kSpPlan + (int)sizeof(SpPlan);
 static_assert(kSpSmemBytes <= 227 * 1024, "shared memory of one CTA");
 
-// Workspace: head {units, pieces}, one record per sequence, then the partials.
-struct SpHead {
-  long long units;
-  int pieces;
+// What the merge needs of a sequence; keys = 0: no shared part.
+struct SpRec {
+  int keys, split;            // shared keys; pieces of a row block
+  int off, blocks;            // the group's first job; row blocks of a kv head
+  int start, members, rank;   // members of the groups before; members of the group; this one's number
   int pad;
 };
-struct SpRec {       // of one sequence; keys = 0: no shared part
-  int keys, tiles, blocks, rank;  // shared keys; units per row block; row blocks per kv head; member number
-  long long off;                  // the group's first unit
-  int start, members;             // members of the groups before; members of the group
-};
-constexpr size_t kSpRecBytes = sizeof(SpHead) + kSpMaxSeqs * sizeof(SpRec);
+constexpr size_t kSpRecBytes = kSpMaxSeqs * sizeof(SpRec);
 
 struct SharedArgs {
   const __nv_bfloat16* q;
@@ -95,7 +94,6 @@ struct SharedArgs {
   int B, Hq, Hkv, G, page, members;  // members: of a row block, kSpRows / G
   long long num_slots;
   float scale_log2;
-  SpHead* head;
   SpRec* rec;
   // own keys (own_keys.cuh)
   int* queue;         // kOwnQueueBytes, zero between calls
@@ -107,21 +105,10 @@ struct SharedArgs {
   long long out_stride;
   float2* first_ml;   // [B * Hq]           pieces that start a row block: rows by group, kv head, member, head
   float* first_o;     // [B * Hq][128]
-  float2* rest_ml;    // [CTAs][kSpRows]    pieces that start inside one: rows of the block
-  float* rest_o;      // [CTAs][kSpRows][128]
+  float2* rest_ml;    // [SMs][kSpRows]     the others, by job: rows of the block
+  float* rest_o;      // [SMs][kSpRows][128]
   unsigned* err;
 };
-
-// First unit of piece c.
-__host__ __device__ __forceinline__ long long sp_piece_start(long long units, int pieces, int c) {
-  return units * c / pieces;
-}
-// The pieces that start strictly inside units (u0, u0 + n): first and behind the last.
-__host__ __device__ __forceinline__ void sp_pieces_inside(long long units, int pieces, long long u0, int n, int& c0,
-                                                          int& c1) {
-  c0 = (int)(((u0 + 1) * pieces + units - 1) / units);
-  c1 = (int)(((u0 + n) * pieces + units - 1) / units);
-}
 
 __device__ __forceinline__ float sp_exp2(float x) {
   float y;
@@ -150,6 +137,32 @@ __device__ __forceinline__ F2 sp_add2(F2 a, F2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
+}
+// One lane of a converged warp, always the same one.
+__device__ __forceinline__ bool sp_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// 2^y of two values on the FMA pipe: n = round(y), 2^n from its bits, 2^(y - n)
+// by the polynomial of degree 4 that is best on [-1/2, 1/2] (its relative error,
+// found by exchange, is 2.7e-6).  Below -127 the result is 0; NaN stays NaN.
+__device__ __forceinline__ F2 sp_exp2_fma(F2 y) {
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: y + kRound has n in its low bits
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y.y) : "f"(-127.f));
+  const F2 t = sp_add2(y, {kRound, kRound});
+  const F2 n = sp_add2(t, {-kRound, -kRound});
+  const F2 f = sp_fma2(n, {-1.f, -1.f}, y);
+  F2 p = {0.00957010220736265f, 0.00957010220736265f};
+  p = sp_fma2(p, f, {0.05591785907745361f, 0.05591785907745361f});
+  p = sp_fma2(p, f, {0.240247443318367f, 0.240247443318367f});
+  p = sp_fma2(p, f, {0.6931217908859253f, 0.6931217908859253f});
+  p = sp_fma2(p, f, {0.9999992847442627f, 0.9999992847442627f});
+  const F2 s = {__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)};
+  return sp_fma2(p, s, {0.f, 0.f});
 }
 __device__ __forceinline__ float sp_max3(float a, float b, float c) {
   float d;
@@ -241,6 +254,35 @@ __device__ __forceinline__ int sp_shared_pages(const SharedArgs& a, int given, i
   return members < 2 ? 0 : min(max(min(given, least), 0) / a.page, a.bt_width);
 }
 
+// Tiles of a piece, chosen by one warp: each lane weighs one number of pieces of
+// the longest prefix by a model of both kernels, fitted to measurements (us, on
+// 148 SMs).  A CTA of this kernel takes about kSpCostJob + kSpCostTile a tile;
+// an SM streams own keys at 60 GB/s, all of them together at 6.1 TB/s, and the
+// own-keys kernel takes the SMs without a job at once and the others when
+// their jobs end.
+constexpr float kSpCostJob = 14.f, kSpCostTile = 2.2f, kSpCostOwn = 10.f;
+__device__ __forceinline__ int sp_choose_piece(const SharedArgs& a, const SpPlan& s, int longest, long long own_keys) {
+  const int lane = threadIdx.x & 31, sms = gridDim.x;
+  const int pieces = lane < 16 ? lane + 1 : 8 * lane - 104;  // 1 .. 16, 24, 32 .. 144
+  const int len = max(1, (longest + pieces - 1) / pieces);
+  float jobs = 0.f;  // (their number can pass 31 bits before it is refused)
+  for (int g = 0; g < a.groups; ++g)
+    if (s.tiles[g] > 0)
+      jobs += (float)((s.cnt[g] + a.members - 1) / a.members * a.Hkv) * (float)((s.tiles[g] + len - 1) / len);
+  const float bytes = (float)own_keys * a.Hkv * 512.f;
+  const float shared = (kSpCostJob + kSpCostTile * len) * ceilf(jobs / sms);
+  const float rate = fminf(fmaxf(sms - jobs, 0.f) * 60e3f, 6.1e6f);     // bytes / us beside the jobs
+  const float left = bytes - fmaxf(shared - kSpCostOwn, 0.f) * rate;     // when they end
+  float cost = left > 0.f ? shared + 2.f + left / 6.1e6f : shared;
+  if (jobs > sms && pieces > 1) cost = 3e38f;  // cut only what fits the SMs
+  // the least cost, and of equals the fewest pieces
+  float best = cost;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  const int who = __ffs(__ballot_sync(0xffffffffu, cost == best)) - 1;
+  return __shfl_sync(0xffffffffu, len, max(who, 0));
+}
+
 // Builds the plan (every CTA the same) in shared memory.  All threads call it.
 __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
   const int tid = threadIdx.x, lane = tid & 31;
@@ -249,11 +291,21 @@ __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
     s.least[g] = 0x7fffffff;
     s.tiles[g] = a.prefix_len[g];
   }
+  if (tid == 0) s.keys = 0;
   __syncthreads();
-  for (int b = tid; b < a.B; b += kSpThreads) {
-    const int g = sp_group_of(a, b, blockIdx.x == 0);
-    s.group[b] = (short)g;
-    if (g >= 0) atomicMin(&s.least[g], a.cu_k[b + 1] - a.cu_k[b]);
+  for (int b0 = 0; b0 < a.B; b0 += kSpThreads) {
+    const int b = b0 + tid;
+    int nk = 0;
+    if (b < a.B) {
+      const int g = sp_group_of(a, b, blockIdx.x == 0);
+      nk = a.cu_q[b + 1] > a.cu_q[b] ? max(a.cu_k[b + 1] - a.cu_k[b], 0) : 0;
+      s.group[b] = (short)g;
+      if (g >= 0) atomicMin(&s.least[g], nk);
+    }
+    unsigned long long sum = nk;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) atomicAdd(&s.keys, sum);
   }
   __syncthreads();
   if (tid < 32) {
@@ -272,40 +324,51 @@ __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
       if (g >= 0 && before == 0) s.cnt[g] = n + __popc(same);
       __syncwarp();
     }
-    // prefix sums of members and units over the groups
-    int members = 0;
-    long long units = 0;
+    // prefixes, then the length of a piece, then first members and jobs
+    int longest = 0;
+    long long shared_keys = 0;
+    for (int g = lane; g < a.groups; g += 32) {
+      const int tiles = sp_shared_pages(a, s.tiles[g], s.cnt[g], s.least[g]) * (a.page / kSpTile);
+      s.tiles[g] = tiles;
+      longest = max(longest, tiles);
+      shared_keys += (long long)s.cnt[g] * tiles * kSpTile;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+      shared_keys += __shfl_xor_sync(0xffffffffu, shared_keys, o);
+    }
+    __syncwarp();
+    const int len = sp_choose_piece(a, s, longest, (long long)s.keys - shared_keys);
+    int members = 0, jobs = 0;
     for (int g0 = 0; g0 < a.groups; g0 += 32) {
       const int g = g0 + lane;
-      int n = 0, tiles = 0;
-      long long u = 0;
+      int n = 0, split = 0, j = 0;
       if (g < a.groups) {
         n = s.cnt[g];
-        tiles = sp_shared_pages(a, s.tiles[g], n, s.least[g]) * (a.page / kSpTile);
-        u = (long long)((n + a.members - 1) / a.members) * a.Hkv * tiles;
+        split = (s.tiles[g] + len - 1) / len;
+        j = (n + a.members - 1) / a.members * a.Hkv * split;
       }
-      int ni = n;
-      long long ui = u;
+      int ni = n, ji = j;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, ni, o);
-        const long long y = __shfl_up_sync(0xffffffffu, ui, o);
+        const int x = __shfl_up_sync(0xffffffffu, ni, o), y = __shfl_up_sync(0xffffffffu, ji, o);
         if (lane >= o) {
           ni += x;
-          ui += y;
+          ji += y;
         }
       }
       if (g < a.groups) {
         s.start[g] = members + ni - n;
-        s.off[g] = units + ui - u;
-        s.tiles[g] = tiles;
+        s.off[g] = jobs + ji - j;
+        s.split[g] = split;
       }
       members += __shfl_sync(0xffffffffu, ni, 31);
-      units += __shfl_sync(0xffffffffu, ui, 31);
+      jobs += __shfl_sync(0xffffffffu, ji, 31);
     }
     if (lane == 0) {
       s.start[a.groups] = members;
-      s.off[a.groups] = units;
+      s.off[a.groups] = jobs;
     }
   }
   __syncthreads();
@@ -314,31 +377,28 @@ __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
   __syncthreads();
 }
 
-// A run of units of one row block.
+// A job: a run of tiles of one row block.
 struct SpSeg {
   int g, h, block;   // group, kv head, row block
   int k0, k1;        // tiles of the prefix
   int rows, nt;      // valid rows; tiles of 128 rows in use
 };
 
-__device__ __forceinline__ SpSeg sp_segment(const SharedArgs& a, const SpPlan& s, long long u, long long u_end) {
-  int lo = 0, hi = a.groups - 1;  // the last group that starts at u or before it
+__device__ __forceinline__ SpSeg sp_segment(const SharedArgs& a, const SpPlan& s, int job) {
+  int lo = 0, hi = a.groups - 1;  // the last group that starts at the job or before it
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (s.off[mid] <= u) lo = mid; else hi = mid - 1;
+    if (s.off[mid] <= job) lo = mid; else hi = mid - 1;
   }
   SpSeg g;
   g.g = lo;
-  const int tiles = s.tiles[lo];
-  const int n = s.start[lo + 1] - s.start[lo];
+  const int n = s.start[lo + 1] - s.start[lo], split = s.split[lo];
   const int blocks = (n + a.members - 1) / a.members;
-  const long long local = u - s.off[lo];
-  const int at = (int)(local / tiles);
-  g.k0 = (int)(local - (long long)at * tiles);
+  const int at = (job - s.off[lo]) / split, piece = job - s.off[lo] - at * split;
+  g.k0 = (int)((long long)s.tiles[lo] * piece / split);
+  g.k1 = (int)((long long)s.tiles[lo] * (piece + 1) / split);
   g.h = at / blocks;
   g.block = at - g.h * blocks;
-  const long long left = u_end - u;
-  g.k1 = left < tiles - g.k0 ? g.k0 + (int)left : tiles;
   g.rows = min(a.members, n - g.block * a.members) * a.G;
   g.nt = g.rows > 128 ? 2 : 1;
   return g;
@@ -361,7 +421,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSpBar);
   uint64_t* full = bars;                   // [kSpSlots]
   uint64_t* empty = bars + kSpSlots;       // [kSpSlots]
-  uint64_t* q_full = bars + 2 * kSpSlots;  // [2] a segment's query rows are in shared memory, O may be overwritten
+  uint64_t* q_full = bars + 2 * kSpSlots;  // [2] a job's query rows are in shared memory, O may be overwritten
   uint64_t* s_full = q_full + 2;           // [2]
   uint64_t* p_full = q_full + 4;           // [2]
   uint64_t* o_done = q_full + 6;           // [2]
@@ -370,7 +430,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 11);
   volatile int* bad = reinterpret_cast<int*>(q_full + 12);  // some page is missing: the softmax looks which
   SpPlan& plan = *reinterpret_cast<SpPlan*>(smem + kSpPlan);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmK);
@@ -390,32 +450,25 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   griddep_wait();
   griddep_launch_dependents();
   sp_build_plan(a, plan);
-  const long long units = plan.off[a.groups];
-  const int pieces = (int)(units < gridDim.x ? units : gridDim.x);
+  const int jobs = plan.off[a.groups];
   if (blockIdx.x == 0) {
     // what the merge needs
-    if (threadIdx.x == 0) {
-      a.head->units = units;
-      a.head->pieces = pieces;
-    }
     for (int b = threadIdx.x; b < a.B; b += kSpThreads) {
       SpRec r{};
       const int g = plan.group[b];
       if (g >= 0 && plan.tiles[g] > 0) {
         r.keys = plan.tiles[g] * kSpTile;
-        r.tiles = plan.tiles[g];
-        r.blocks = (plan.start[g + 1] - plan.start[g] + a.members - 1) / a.members;
-        r.rank = plan.rank[b];
+        r.split = plan.split[g];
         r.off = plan.off[g];
         r.start = plan.start[g];
         r.members = plan.start[g + 1] - plan.start[g];
+        r.blocks = (r.members + a.members - 1) / a.members;
+        r.rank = plan.rank[b];
       }
       a.rec[b] = r;
     }
   }
-  if ((int)blockIdx.x >= pieces) return;  // the whole CTA, before any TMEM
-  const long long u_beg = sp_piece_start(units, pieces, blockIdx.x);
-  const long long u_end = sp_piece_start(units, pieces, blockIdx.x + 1);
+  if ((int)blockIdx.x >= jobs) return;  // the whole CTA, before any TMEM
 
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -433,8 +486,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     if (warp == 0 && lane == 0) {
       int it = 0;      // loads issued; load it is in slot it % kSpSlots
       bool ok = true;
-      for (long long u = u_beg; ok && u < u_end;) {
-        const SpSeg g = sp_segment(a, plan, u, u_end);
+      for (int job = blockIdx.x; ok && job < jobs; job += gridDim.x) {
+        const SpSeg g = sp_segment(a, plan, job);
         const int leader = plan.member[plan.start[g.g]];
         for (int k = g.k0; ok && k < g.k1; ++k) {
           long long row = sp_tile_row(a, leader, k);
@@ -457,75 +510,88 @@ __global__ void __launch_bounds__(kSpThreads, 1)
             ++it;
           }
         }
-        u += g.k1 - g.k0;
       }
       // every load has landed before the CTA may end (a wait that gave up leaves some unread)
       for (int i = it > kSpSlots ? it - kSpSlots : 0; i < it; ++i)
         mbar_wait(&full[i % kSpSlots], (uint32_t)(i / kSpSlots) & 1u, a.err);
     }
-    // ---- MMA issuer
-    if (warp == 1 && lane == 0) {
+    // ---- MMA issuer: the whole warp walks the loop, so that descriptors live in
+    // uniform registers, and one elected lane issues
+    if (warp == 1) {
       const uint32_t idesc_s = umma_idesc_bf16(128, kSpTile);
       const uint32_t idesc_o = umma_idesc_bf16(128, 128) | (1u << 16);  // B (V) MN-major
+      // descriptors count in 16 bytes: 2048 a ring slot or Q tile, 1024 a half of the dims
+      const uint64_t dq = umma_desc_sw128(base + kSpQ), dk = umma_desc_sw128(base + kSpRing),
+                     dv = umma_desc_sw128_mn(base + kSpRing, 16384u);
+      const bool leader = sp_elect();
       int it = 0, seg[2] = {0, 0}, step[2] = {0, 0};
       bool ok = true;
       auto wait_slot = [&](int i) { return mbar_wait(&full[i % kSpSlots], (uint32_t)(i / kSpSlots) & 1u, a.err); };
       auto scores = [&](int t, int i) {  // S_t = Q_t K^T, K in load i
-        const uint32_t qb = base + kSpQ + (uint32_t)t * 32768u;
-        const uint32_t kb = base + kSpRing + (uint32_t)(i % kSpSlots) * 32768u;
+        const uint64_t q = dq + (uint32_t)t * 2048u, k = dk + (uint32_t)(i % kSpSlots) * 2048u;
+        if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const uint32_t o = (uint32_t)(kk >> 2) * 16384u + (uint32_t)(kk & 3) * 32u;
-          tc_mma_f16(tmem + (uint32_t)t * 128u, umma_desc_sw128(qb + o), umma_desc_sw128(kb + o), idesc_s,
-                     kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t o = (uint32_t)(kk >> 2) * 1024u + (uint32_t)(kk & 3) * 2u;
+            tc_mma_f16(tmem + (uint32_t)t * 128u, q + o, k + o, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[t]);
         }
-        tc_commit(&s_full[t]);
       };
       auto values = [&](int t, int i, int half, bool acc) {  // O_t (+)= P_t V over 64 keys, V in load i
-        const uint32_t vb = base + kSpRing + (uint32_t)(i % kSpSlots) * 32768u;
+        const uint64_t v = dv + (uint32_t)(i % kSpSlots) * 2048u;
+        if (leader) {
 #pragma unroll
-        for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-          tc_mma_f16_ts(tmem + 256u + (uint32_t)t * 128u, tmem + (uint32_t)t * 128u + (uint32_t)kk * 8u,
-                        umma_desc_sw128_mn(vb + (uint32_t)kk * 2048u, 16384u), idesc_o, (acc || kk > 0) ? 1u : 0u);
+          for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+            tc_mma_f16_ts(tmem + 256u + (uint32_t)t * 128u, tmem + (uint32_t)t * 128u + (uint32_t)kk * 8u,
+                          v + (uint32_t)kk * 128u, idesc_o, (acc || kk > 0) ? 1u : 0u);
+        }
       };
-      for (long long u = u_beg; ok && u < u_end;) {
-        const SpSeg g = sp_segment(a, plan, u, u_end);
+      auto commit = [&](uint64_t* bar) {
+        if (leader) tc_commit(bar);
+      };
+      for (int job = blockIdx.x; ok && job < jobs; job += gridDim.x) {
+        const SpSeg g = sp_segment(a, plan, job);
         // the first scores of both tiles
-        if (!wait_slot(it)) break;
+        ok = wait_slot(it);
         for (int t = 0; ok && t < g.nt; ++t) {
           ok = mbar_wait(&q_full[t], (uint32_t)seg[t] & 1u, a.err);
+          ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
           if (ok) scores(t, it);
         }
-        if (!ok) break;
-        tc_commit(&empty[it % kSpSlots]);
-        for (int k = g.k0; ok && k < g.k1; ++k, it += 2) {
+        if (!__all_sync(0xffffffffu, ok)) break;
+        commit(&empty[it % kSpSlots]);
+        for (int k = g.k0; k < g.k1; ++k, it += 2) {
           const bool more = k + 1 < g.k1;
           ok = wait_slot(it + 1) && (!more || wait_slot(it + 2));
-          for (int t = 0; ok && t < g.nt; ++t) {
-            ok = mbar_wait(&p_half[t], (uint32_t)step[t] & 1u, a.err);
+          for (int t = 0; t < g.nt; ++t) {
+            ok = ok && mbar_wait(&p_half[t], (uint32_t)step[t] & 1u, a.err);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             values(t, it + 1, 0, k > g.k0);
             ok = mbar_wait(&p_full[t], (uint32_t)step[t] & 1u, a.err);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             ++step[t];
             tc_fence_after();
             values(t, it + 1, 1, true);
             // S_t's next scores overwrite P_t: MMAs of one thread run in the order of issue
             if (more) scores(t, it + 2);
-            else tc_commit(&o_done[t]);
+            else commit(&o_done[t]);
           }
           if (!ok) break;
-          tc_commit(&empty[(it + 1) % kSpSlots]);
-          if (more) tc_commit(&empty[(it + 2) % kSpSlots]);
+          commit(&empty[(it + 1) % kSpSlots]);
+          if (more) commit(&empty[(it + 2) % kSpSlots]);
         }
+        if (!ok) break;
         for (int t = 0; t < g.nt; ++t) ++seg[t];
-        u += g.k1 - g.k0;
       }
       // every MMA issued has completed before TMEM can be released
-      tc_commit(drain);
+      commit(drain);
       mbar_wait(drain, 0u, a.err);
+      __syncwarp();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSpRegsSoftmax));
@@ -537,9 +603,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     const uint32_t ts = tmem + lanes + (uint32_t)t * 128u, to = ts + 256u;
     int seg = 0, step = 0;
     bool ok = true;
-    for (long long u = u_beg; ok && u < u_end;) {
-      const SpSeg g = sp_segment(a, plan, u, u_end);
-      u += g.k1 - g.k0;
+    for (int job = blockIdx.x; ok && job < jobs; job += gridDim.x) {
+      const SpSeg g = sp_segment(a, plan, job);
       if (t >= g.nt) continue;
       const int m0 = plan.start[g.g] + g.block * a.members;  // first member of the block
       uint8_t* qrows = smem + kSpQ + t * 32768 + q4 * 4096;  // this warp's 32 rows (64 dims; the others 16 KB on)
@@ -547,18 +612,21 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         // the rows in the swizzled K-major layout of the MMA, two rows of 256 bytes a load
         const int r = t * 128 + row;  // row of the block: member r / G, head r % G (zeros behind the last member)
         const int i = r / a.G;
-        const bool valid = r < g.rows;
-        const long long from = valid ? (long long)a.cu_q[plan.member[m0 + i]] * a.q_stride + (g.h * a.G + r - i * a.G) * 128
-                                     : -1;
+        // (every lane loads, from the block's first row where there is none: a
+        // load under a condition would be waited for before the next one)
+        const long long from = r < g.rows ? (long long)a.cu_q[plan.member[m0 + i]] * a.q_stride +
+                                                (g.h * a.G + r - i * a.G) * 128
+                                          : (long long)a.cu_q[plan.member[m0]] * a.q_stride + g.h * a.G * 128;
         uint4 v[16];
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
           const long long at = __shfl_sync(0xffffffffu, from, 2 * c + (lane >> 4));
-          v[c] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.q + at) + (lane & 15)) : make_uint4(0u, 0u, 0u, 0u);
+          v[c] = __ldg(reinterpret_cast<const uint4*>(a.q + at) + (lane & 15));
         }
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
           const int rr = 2 * c + (lane >> 4), ch = lane & 15;
+          if (t * 128 + q4 * 32 + rr >= g.rows) v[c] = make_uint4(0u, 0u, 0u, 0u);
           *reinterpret_cast<uint4*>(qrows + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = v[c];
         }
         fence_proxy_async_smem();
@@ -614,7 +682,12 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const F2 y = sp_fma2({s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]}, scale2, minus);
-            const F2 e = {sp_exp2(y.x), sp_exp2(y.y)};
+            // three pairs of eight on the FMA pipe: the exponential unit alone
+            // would take as long as the products
+            const bool fma = (i & 7) == 1 || (i & 7) == 4 || (i & 7) == 6;
+            F2 e;
+            if (fma) e = sp_exp2_fma(y);
+            else e = {sp_exp2(y.x), sp_exp2(y.y)};
             sum[i & 3] = sp_add2(sum[i & 3], e);
             pk[i] = pack_bf16x2(e.x, e.y);
           }
@@ -629,7 +702,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         l += rs.x + rs.y;
       }
       if (!ok) break;
-      // ---- the segment's partial
+      // ---- the job's partial
       ok = mbar_wait(&o_done[t], (uint32_t)seg & 1u, a.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -638,7 +711,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       const bool first = g.k0 == 0;
       const size_t at = first ? ((size_t)plan.start[g.g] * a.Hkv +
                                  (size_t)g.h * (plan.start[g.g + 1] - plan.start[g.g]) + g.block * a.members) * a.G
-                              : (size_t)blockIdx.x * kSpRows;
+                              : (size_t)job * kSpRows;  // (cut only when there are no more jobs than SMs)
       const int r0 = t * 128 + q4 * 32;  // this warp's first row of the block
       if (r0 + lane < g.rows) (first ? a.first_ml : a.rest_ml)[at + r0 + lane] = make_float2(m, l);
       float* po = (first ? a.first_o : a.rest_o) + (at + r0) * 128;
