@@ -56,6 +56,22 @@ constexpr int kOwnSmemBytes = 1024 + kOwnWarps * kOwnWarpBytes + (int)sizeof(Own
 static_assert(kOwnSmemBytes <= 227 * 1024, "shared memory of one CTA");
 static_assert(2 * kSpMaxGroups * 4 <= kOwnWarps * kOwnWarpBytes, "the counts fit the rings");
 
+// Tiled load of keys that no one else will read: they leave L2 first, before
+// the shared prefixes, the partials and the kernels' own instructions.
+__device__ __forceinline__ uint64_t own_read_once() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void own_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t c0, int32_t c1,
+                                            int32_t c2, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+      : "memory");
+}
+
 // byte offset of 16-byte chunk ch (0..15 over 128 dims) of row r in a tile of [2 halves][rows][128 B]
 __device__ __forceinline__ uint32_t own_at(int half_bytes, int r, int ch) {
   return (uint32_t)((ch >> 3) * half_bytes + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
@@ -159,6 +175,7 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
     // ---- producer
     const int items = total * a.Hkv;
     const int q_rows = min(a.Hq, 8);
+    const uint64_t once = own_read_once();
     int it = 0;  // tiles issued; tile it is in stage it % kOwnStages
     bool ok = true;
     auto stage_free = [&]() {
@@ -212,10 +229,10 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
           const uint32_t at = smem_u32(ring) + (uint32_t)st * kOwnStageBytes, bar = smem_u32(&s.full[w][st]);
           const int r = there ? (int)row : 0;
           mbar_arrive_expect_tx(&s.full[w][st], 4 * 4096 + (k == 0 ? 256 * q_rows : 0));
-          tma_load_3d(at + kOwnK, &tmK, bar, 0, h, r);
-          tma_load_3d(at + kOwnK + 4096, &tmK, bar, 64, h, r);
-          tma_load_3d(at + kOwnV, &tmV, bar, 0, h, r);
-          tma_load_3d(at + kOwnV + 4096, &tmV, bar, 64, h, r);
+          own_load_3d(at + kOwnK, &tmK, bar, 0, h, r, once);
+          own_load_3d(at + kOwnK + 4096, &tmK, bar, 64, h, r, once);
+          own_load_3d(at + kOwnV, &tmV, bar, 0, h, r, once);
+          own_load_3d(at + kOwnV + 4096, &tmV, bar, 64, h, r, once);
           if (k == 0) {
             tma_load_3d(at + kOwnQ, &tmQ, bar, 0, h * a.G, d.qrow);
             tma_load_3d(at + kOwnQ + 1024, &tmQ, bar, 64, h * a.G, d.qrow);
