@@ -1576,6 +1576,22 @@ SharedLayout shared_layout(int num_sms, int seqs, int max_seqlen_k, int Hq, int 
   return l;
 }
 
+// The softmax warps raise their register count to what the launch has to give:
+// a build in which the kernel takes fewer registers must not start.
+int check_prefix_registers() {
+  static int regs = 0;
+  std::lock_guard<std::mutex> lock(g_host_mutex);
+  if (regs == 0) {
+    cudaFuncAttributes f{};
+    const cudaError_t e = cudaFuncGetAttributes(&f, shared_prefix_kernel);
+    if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix: %s", cudaGetErrorString(e));
+    regs = f.numRegs;
+  }
+  if (regs < kSpRegsLaunch)
+    return fail(B200_ERR_UNSUPPORTED, "shared_prefix: built with %d registers a thread, %d needed", regs, kSpRegsLaunch);
+  return B200_OK;
+}
+
 // Launch that may begin while the one before it in the stream still runs (see griddep_wait).
 template <typename... KArgs, typename... Args>
 cudaError_t launch_overlapped(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t st, Args... args) {
@@ -1662,6 +1678,7 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   // the shared part
   if (int r = make_tmap_3d(&tmK, k_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kSpTile)) return r;
   if (int r = make_tmap_3d(&tmV, v_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kSpTile)) return r;
+  if (int r = check_prefix_registers()) return r;
   if (int r = ensure_smem(ds, 32u, shared_prefix_kernel, kSpSmemBytes)) return r;
   cudaError_t e = launch_ex(shared_prefix_kernel, dim3(ds->num_sms), dim3(kSpThreads), kSpSmemBytes, st, nullptr, 0,
                             tmK, tmV, s);

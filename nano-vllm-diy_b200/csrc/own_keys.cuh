@@ -35,7 +35,7 @@ constexpr int kOwnThreads = kOwnWarps * 64;
 constexpr int kOwnK = 0, kOwnV = 8192, kOwnQ = 16384;
 constexpr int kOwnStageBytes = 18432;
 constexpr int kOwnWarpBytes = kOwnStages * kOwnStageBytes;
-constexpr int kOwnQueueBytes = 256;  // {next item, producers out of the queue}: zero between calls
+constexpr int kOwnQueueBytes = 256;  // {next item, producers out of the queue, items + 1}: zero between calls
 
 struct OwnTile {
   int b, h, c, qrow;
@@ -77,6 +77,15 @@ __device__ __forceinline__ uint32_t own_at(int half_bytes, int r, int ch) {
   return (uint32_t)((ch >> 3) * half_bytes + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
 }
 
+// `n` producers are done with the queue; the last of all resets it for the next call.
+__device__ __forceinline__ void own_leave(const SharedArgs& a, int n) {
+  if (atomicAdd(&a.queue[1], n) + n == (int)gridDim.x * kOwnWarps) {
+    atomicExch(&a.queue[0], 0);
+    atomicExch(&a.queue[2], 0);
+    atomicExch(&a.queue[1], 0);
+  }
+}
+
 __global__ void __launch_bounds__(kOwnThreads, 1)
     own_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ CUtensorMap tmQ, const SharedArgs a) {
@@ -93,6 +102,22 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
     tma_prefetch_desc(&tmQ);
+  }
+  // A CTA that comes late (its SM had a job of the prefix) and finds the queue
+  // empty needs no plan.
+  {
+    __shared__ int s_late;
+    if (tid == 0) {
+      const int items = *reinterpret_cast<volatile int*>(&a.queue[2]) - 1;
+      s_late = items >= 0 && *reinterpret_cast<volatile int*>(&a.queue[0]) >= items;
+    }
+    __syncthreads();
+    if (s_late) {
+      if (tid == 0) own_leave(a, kOwnWarps);
+      griddep_launch_dependents();
+      griddep_wait();
+      return;
+    }
   }
   // ---- plan (every CTA the same): shared keys, then the prefix sum of items.
   // The inputs are older than the prefix kernel, which waited for them.
@@ -174,6 +199,10 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
   if (warp >= kOwnWarps) {
     // ---- producer
     const int items = total * a.Hkv;
+    if (w == 0 && lane == 0) {  // for late CTAs; in place before this thread leaves the queue
+      atomicExch(&a.queue[2], items + 1);
+      __threadfence();
+    }
     const int q_rows = min(a.Hq, 8);
     const uint64_t once = own_read_once();
     int it = 0;  // tiles issued; tile it is in stage it % kOwnStages
@@ -242,11 +271,7 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
       }
     }
     if (lane == 0) {
-      // the last producer out of the queue resets it for the next call
-      if (atomicAdd(&a.queue[1], 1) == (int)gridDim.x * kOwnWarps - 1) {
-        atomicExch(&a.queue[0], 0);
-        atomicExch(&a.queue[1], 0);
-      }
+      own_leave(a, 1);
       if (ok && stage_free()) {
         s.tile[w][it % kOwnStages].ntok = -1;
         mbar_arrive(&s.full[w][it % kOwnStages]);
@@ -414,7 +439,7 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
 // ---------------------------------------------------------------------------
 constexpr int kMergeWarps = 8;
 
-__global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(const SharedArgs a) {
+__global__ void __launch_bounds__(kMergeWarps * 32, 5) shared_merge_kernel(const SharedArgs a) {
   griddep_wait();
   griddep_launch_dependents();
   const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;

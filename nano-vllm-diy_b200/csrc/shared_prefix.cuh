@@ -283,9 +283,19 @@ __device__ __forceinline__ int sp_choose_piece(const SharedArgs& a, const SpPlan
   return __shfl_sync(0xffffffffu, len, max(who, 0));
 }
 
+// The MMA warp, which allocates TMEM, and the softmax warps, which use it.
+__device__ __forceinline__ void sp_bar_tmem() { asm volatile("bar.sync 1, 288;" ::: "memory"); }
+
 // Builds the plan (every CTA the same) in shared memory.  All threads call it.
 __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
   const int tid = threadIdx.x, lane = tid & 31;
+  auto row = [&](int b, int& nk) {  // group and keys of a row
+    nk = 0;
+    if (b >= a.B) return -1;
+    nk = a.cu_q[b + 1] > a.cu_q[b] ? max(a.cu_k[b + 1] - a.cu_k[b], 0) : 0;
+    return sp_group_of(a, b, blockIdx.x == 0);
+  };
+  int nk, g0 = row(tid, nk);  // (loaded beside the prefix lengths: one round trip)
   for (int g = tid; g < a.groups; g += kSpThreads) {
     s.cnt[g] = 0;
     s.least[g] = 0x7fffffff;
@@ -295,13 +305,9 @@ __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
   __syncthreads();
   for (int b0 = 0; b0 < a.B; b0 += kSpThreads) {
     const int b = b0 + tid;
-    int nk = 0;
-    if (b < a.B) {
-      const int g = sp_group_of(a, b, blockIdx.x == 0);
-      nk = a.cu_q[b + 1] > a.cu_q[b] ? max(a.cu_k[b + 1] - a.cu_k[b], 0) : 0;
-      s.group[b] = (short)g;
-      if (g >= 0) atomicMin(&s.least[g], nk);
-    }
+    if (b0 > 0) g0 = row(b, nk);
+    if (b < a.B) s.group[b] = (short)g0;
+    if (g0 >= 0) atomicMin(&s.least[g0], nk);
     unsigned long long sum = nk;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -451,37 +457,28 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   griddep_launch_dependents();
   sp_build_plan(a, plan);
   const int jobs = plan.off[a.groups];
-  if (blockIdx.x == 0) {
-    // what the merge needs
-    for (int b = threadIdx.x; b < a.B; b += kSpThreads) {
-      SpRec r{};
-      const int g = plan.group[b];
-      if (g >= 0 && plan.tiles[g] > 0) {
-        r.keys = plan.tiles[g] * kSpTile;
-        r.split = plan.split[g];
-        r.off = plan.off[g];
-        r.start = plan.start[g];
-        r.members = plan.start[g + 1] - plan.start[g];
-        r.blocks = (r.members + a.members - 1) / a.members;
-        r.rank = plan.rank[b];
-      }
-      a.rec[b] = r;
-    }
-  }
-  if ((int)blockIdx.x >= jobs) return;  // the whole CTA, before any TMEM
-
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // S / P of tile t at t * 128, O of tile t at 256 + t * 128
+  if ((int)blockIdx.x >= jobs && blockIdx.x > 0) return;  // the whole CTA, before any TMEM
   const uint32_t base = smem_u32(smem);
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSpRegsIssue));
+    // ---- what the merge needs
+    if (blockIdx.x == 0 && warp >= 2) {
+      for (int b = threadIdx.x - 64; b < a.B; b += 64) {
+        SpRec r{};
+        const int g = plan.group[b];
+        if (g >= 0 && plan.tiles[g] > 0) {
+          r.keys = plan.tiles[g] * kSpTile;
+          r.split = plan.split[g];
+          r.off = plan.off[g];
+          r.start = plan.start[g];
+          r.members = plan.start[g + 1] - plan.start[g];
+          r.blocks = (r.members + a.members - 1) / a.members;
+          r.rank = plan.rank[b];
+        }
+        a.rec[b] = r;
+      }
+    }
     // ---- producer
     if (warp == 0 && lane == 0) {
       int it = 0;      // loads issued; load it is in slot it % kSpSlots
@@ -518,6 +515,12 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     // ---- MMA issuer: the whole warp walks the loop, so that descriptors live in
     // uniform registers, and one elected lane issues
     if (warp == 1) {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+      tc_fence_before();
+      sp_bar_tmem();
+      tc_fence_after();
+      const uint32_t tmem = *tmem_slot;
       const uint32_t idesc_s = umma_idesc_bf16(128, kSpTile);
       const uint32_t idesc_o = umma_idesc_bf16(128, 128) | (1u << 16);  // B (V) MN-major
       // descriptors count in 16 bytes: 2048 a ring slot or Q tile, 1024 a half of the dims
@@ -599,8 +602,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     const int t = warp >= 8;
     const int q4 = warp & 3;             // TMEM lane quarter of this warp
     const int row = q4 * 32 + lane;      // of the tile
-    const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
-    const uint32_t ts = tmem + lanes + (uint32_t)t * 128u, to = ts + 256u;
+    uint32_t ts = 0, to = 0;             // S / P and O of the row, once TMEM is allocated
+    bool have_tmem = false;
     int seg = 0, step = 0;
     bool ok = true;
     for (int job = blockIdx.x; ok && job < jobs; job += gridDim.x) {
@@ -622,6 +625,13 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         for (int c = 0; c < 16; ++c) {
           const long long at = __shfl_sync(0xffffffffu, from, 2 * c + (lane >> 4));
           v[c] = __ldg(reinterpret_cast<const uint4*>(a.q + at) + (lane & 15));
+        }
+        if (!have_tmem) {
+          sp_bar_tmem();  // (while the rows are on their way)
+          tc_fence_after();
+          ts = *tmem_slot + ((uint32_t)(q4 * 32) << 16) + (uint32_t)t * 128u;
+          to = ts + 256u;
+          have_tmem = true;
         }
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
@@ -739,12 +749,13 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         __syncwarp();
       }
     }
+    if (!have_tmem) sp_bar_tmem();  // (no job had rows for these warps: the barrier still counts them)
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(*tmem_slot, 512);
   }
 }
 
