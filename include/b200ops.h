@@ -304,7 +304,7 @@ int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, i
  *    counts as -1 and flags B200_DEVERR_BAD_INDEX.
  *  - The other arguments are b200_paged_attention's.  A live sequence without
  *    keys gives zeros; rows with q length <= 0 (padding) are left alone.
- *  - B <= 1024, num_groups <= 1024, Hq / Hkv <= 8, page a multiple of 256,
+ *  - B <= 1024, num_groups <= 512, Hq / Hkv <= 8, page a multiple of 256,
  *    softmax_scale > 0.
  *  - workspace: b200_shared_prefix_workspace_bytes(B, max_seqlen_k, Hq, Hkv) bytes,
  *    256-byte aligned, its first 256 bytes zero before the first call (they

@@ -1661,7 +1661,10 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   s.cu_q = cu_seqlens_q; s.cu_k = cu_seqlens_k;
   s.block_tables = block_tables; s.bt_stride = bt_stride; s.bt_width = bt_width;
   s.prefix_group = prefix_group; s.prefix_len = prefix_len; s.groups = num_groups;
-  s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.G = G; s.page = page; s.members = kSpRows / G;
+  s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.G = G; s.page = page;
+  s.members = kSpRows / G;
+  const char* share = getenv("B200_SHARED_PREFIX");
+  s.always = share && std::strcmp(share, "always") == 0;
   s.num_slots = num_slots; s.scale_log2 = softmax_scale * 1.4426950408889634f;
   s.rec = reinterpret_cast<SpRec*>(ws + l.rec);
   s.queue = static_cast<int*>(workspace);
@@ -1695,7 +1698,9 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
   if (int r = check_launch("own_keys_kernel")) return r;
   // the parts of each row
-  e = launch_overlapped(shared_merge_kernel, (B * Hq + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, st, s);
+  const int rows = B * Hq;
+  e = launch_overlapped(rows <= ds->num_sms * 24 ? shared_merge_kernel<8> : shared_merge_kernel<4>,
+                        (rows + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, st, s);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
   return check_launch("shared_merge_kernel");
 }

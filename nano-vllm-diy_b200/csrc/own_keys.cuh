@@ -54,7 +54,7 @@ struct OwnPlan {
 };
 constexpr int kOwnSmemBytes = 1024 + kOwnWarps * kOwnWarpBytes + (int)sizeof(OwnPlan);
 static_assert(kOwnSmemBytes <= 227 * 1024, "shared memory of one CTA");
-static_assert(2 * kSpMaxGroups * 4 <= kOwnWarps * kOwnWarpBytes, "the counts fit the rings");
+static_assert(2 * kSpMaxGroups * 4 + 8 <= kOwnWarps * kOwnWarpBytes, "the counts fit the rings");
 
 // Tiled load of keys that no one else will read: they leave L2 first, before
 // the shared prefixes, the partials and the kernels' own instructions.
@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
   {
     int* cnt = reinterpret_cast<int*>(smem);  // in the rings, before their first load
     int* least = cnt + kSpMaxGroups;
-    sp_count_groups(a, cnt, least, kOwnThreads);
+    unsigned long long* all = reinterpret_cast<unsigned long long*>(least + kSpMaxGroups);
+    sp_count_groups(a, cnt, least, all, nullptr, kOwnThreads);
     const int per = (a.B + kOwnThreads - 1) / kOwnThreads;
     const int beg = min(a.B, tid * per), end = min(a.B, beg + per);
     long long keys = 0;
@@ -434,12 +435,14 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
 // ---------------------------------------------------------------------------
 // The parts of a row of attention with shared prefixes: the prefix's pieces,
 // then the items of the sequence's own keys, always in that order.  One warp
-// per (sequence, query head), 4 dims a lane, four parts in flight: the parts
-// come from L2, so it is latency that counts, and there is a warp for every row.
+// per (sequence, query head), 4 dims a lane.  The parts come from L2, so it is
+// latency that counts: kFlight parts are in flight at once, 8 where few rows
+// leave the registers for it, 4 where more resident warps are worth more.
 // ---------------------------------------------------------------------------
-constexpr int kMergeWarps = 8;
+constexpr int kMergeWarps = 4;
 
-__global__ void __launch_bounds__(kMergeWarps * 32, 5) shared_merge_kernel(const SharedArgs a) {
+template <int kFlight>
+__global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 10) shared_merge_kernel(const SharedArgs a) {
   griddep_wait();
   griddep_launch_dependents();
   const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -456,11 +459,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32, 5) shared_merge_kernel(const
   const int n = pieces + own;
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n; i0 += 4) {
-    float2 ml[4];
-    float4 o[4];
+  for (int i0 = 0; i0 < n; i0 += kFlight) {
+    float2 ml[kFlight];
+    float4 o[kFlight];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kFlight; ++u) {
       const int i = i0 + u;
       const float2* pm;
       const float* po;
@@ -477,7 +480,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32, 5) shared_merge_kernel(const
       o[u] = i < n ? __ldcg(reinterpret_cast<const float4*>(po) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kFlight; ++u) {
       if (ml[u].y == 0.f) continue;  // no key there, or none of a finite score
       const float mn = fmaxf(M, ml[u].x);
       const float s = fast_exp2(M - mn), w = fast_exp2(ml[u].x - mn);

@@ -40,10 +40,10 @@
 namespace b200 {
 
 constexpr int kSpMaxSeqs = 1024;
-constexpr int kSpMaxGroups = 1024;
-constexpr int kSpRows = 256;     // rows of a block: two tiles of 128
-constexpr int kSpTile = 128;     // keys of a unit
-constexpr int kSpSlots = 4;      // ring slots of 32 KB (K, V, K, V, ...)
+constexpr int kSpMaxGroups = 512;  // groups of two at least
+constexpr int kSpTile = 128;       // keys of a tile
+constexpr int kSpRows = 256;       // rows of a block: two tiles of 128
+constexpr int kSpSlots = 4;        // ring slots of 32 KB (K, V, K, V)
 constexpr int kSpThreads = 384;
 // registers: 168 a thread at launch (64 K over 12 warps), then 88 for the first
 // warpgroup and 208 for the softmax: 128 x (88 + 208 + 208) = 384 x 168
@@ -53,23 +53,28 @@ constexpr float kSpLazy = 8.f;
 constexpr int kSpQ = 0;                            // [2 tiles][2 dim halves][128 rows][128 B]
 constexpr int kSpRing = 65536;
 constexpr int kSpBar = kSpRing + kSpSlots * 32768;
-constexpr int kSpPlan = kSpBar + 256;
+constexpr int kSpPlanAt = kSpBar + 256;
 
 // The groups of a call, in shared memory.
 struct SpPlan {
-  unsigned long long keys;          // of all live sequences
   int off[kSpMaxGroups + 1];        // first job of each group
-  int start[kSpMaxGroups + 1];      // first member
-  int split[kSpMaxGroups];          // pieces of a row block
+  int tiles[kSpMaxGroups];          // 128-key tiles of the prefix (0: nothing shared)
+  short start[kSpMaxGroups + 1];    // first member
+  short split[kSpMaxGroups];        // pieces of a row block
+  short member[kSpMaxSeqs];         // sequences by group, in batch order
+};
+// Only while the plan is made; lies in the ring, before its first load.
+struct SpDraft {
+  unsigned long long keys;          // of all live sequences
   int cnt[kSpMaxGroups];
   int least[kSpMaxGroups];          // shortest member (keys)
-  int tiles[kSpMaxGroups];          // 128-key tiles of the prefix (0: nothing shared)
-  short member[kSpMaxSeqs];         // sequences by group, in batch order
   short group[kSpMaxSeqs];
   short rank[kSpMaxSeqs];
+  short seen[kSpMaxGroups];         // members numbered so far
 };
-constexpr int kSpSmemBytes = 1024 + kSpPlan + (int)sizeof(SpPlan);
+constexpr int kSpSmemBytes = 1024 + kSpPlanAt + (int)sizeof(SpPlan);
 static_assert(kSpSmemBytes <= 227 * 1024, "shared memory of one CTA");
+static_assert(sizeof(SpDraft) <= kSpSlots * 32768, "the draft fits the ring");
 
 // What the merge needs of a sequence; keys = 0: no shared part.
 struct SpRec {
@@ -91,6 +96,7 @@ struct SharedArgs {
   const int* prefix_group;  // [B], -1: none
   const int* prefix_len;    // [groups]
   int groups;
+  int always;               // share whatever it costs
   int B, Hq, Hkv, G, page, members;  // members: of a row block, kSpRows / G
   long long num_slots;
   float scale_log2;
@@ -221,6 +227,13 @@ __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, 
       : "memory");
 }
 
+// a / b for 0 <= a < 2^24 and b > 0: the float quotient is off by one at most.
+__device__ __forceinline__ int sp_div(int a, int b) {
+  int q = (int)__fdiv_rn((float)a, (float)b);
+  const int r = a - q * b;
+  return q + (r >= b) - (r < 0);
+}
+
 // The group that sequence b counts in (-1: none): live rows only.  `flag`: report what is out of range.
 __device__ __forceinline__ int sp_group_of(const SharedArgs& a, int b, bool flag = false) {
   const int g = a.prefix_group[b];
@@ -232,26 +245,53 @@ __device__ __forceinline__ int sp_group_of(const SharedArgs& a, int b, bool flag
   return nq < 1 || nk <= 0 ? -1 : g;  // padding rows of a captured batch, rows without keys
 }
 
-// Members and shortest member (keys) of each group.  All `threads` threads of the CTA call it.
-__device__ __forceinline__ void sp_count_groups(const SharedArgs& a, int* cnt, int* least, int threads) {
-  for (int g = threadIdx.x; g < a.groups; g += threads) {
-    cnt[g] = 0;
-    least[g] = 0x7fffffff;
+// Groups, their members and shortest member (keys), and the keys of all live
+// sequences.  All `threads` threads of the CTA call it; `group` may be null.
+__device__ __forceinline__ void sp_count_groups(const SharedArgs& a, int* cnt, int* least, unsigned long long* keys,
+                                                short* group, int threads) {
+  const int tid = threadIdx.x;
+  auto row = [&](int b, int& nk) {
+    nk = 0;
+    if (b >= a.B) return -1;
+    nk = a.cu_q[b + 1] > a.cu_q[b] ? max(a.cu_k[b + 1] - a.cu_k[b], 0) : 0;
+    return sp_group_of(a, b, group != nullptr && blockIdx.x == 0);
+  };
+  int nk, g = row(tid, nk);  // (the loads of the first rows are on their way during the barrier)
+  for (int i = tid; i < a.groups; i += threads) {
+    cnt[i] = 0;
+    least[i] = 0x7fffffff;
   }
+  if (tid == 0) *keys = 0;
   __syncthreads();
-  for (int b = threadIdx.x; b < a.B; b += threads) {
-    const int g = sp_group_of(a, b);
+  for (int b0 = 0; b0 < a.B; b0 += threads) {
+    if (b0 > 0) g = row(b0 + tid, nk);
+    if (group != nullptr && b0 + tid < a.B) group[b0 + tid] = (short)g;
     if (g >= 0) {
       atomicAdd(&cnt[g], 1);
-      atomicMin(&least[g], a.cu_k[b + 1] - a.cu_k[b]);
+      atomicMin(&least[g], nk);
     }
+    unsigned long long sum = nk;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((tid & 31) == 0 && sum > 0) atomicAdd(keys, sum);
   }
   __syncthreads();
 }
 
-// Pages of a group's prefix that count: whole ones that every member sees; a group of one shares none.
+// Pages of a group's prefix that count: whole ones that every member sees.  The
+// prefix is shared where that pays: reading a tile (64 KB) once instead of once
+// a member saves 10.7 ns of HBM's time at 6.1 TB/s, and a job costs an SM about
+// 11 us and 2.15 us a tile.  So pairs never share, four members from 5 tiles on,
+// eight from 2 (measured: 64 pairs behind 512 keys 101 us shared and 74 not, 16
+// groups of 4 behind 512 38 and 33; 64 groups of 4 behind 2k 146 and 223).
 __device__ __forceinline__ int sp_shared_pages(const SharedArgs& a, int given, int members, int least) {
-  return members < 2 ? 0 : min(max(min(given, least), 0) / a.page, a.bt_width);
+  if (members < 2) return 0;
+  const int pages = min(max(min(given, least), 0) / a.page, a.bt_width);
+  // (in whole numbers: both kernels have to come to the same answer)
+  const long long tiles = (long long)pages * (a.page / kSpTile);
+  const long long saved = (members - 1) * tiles * 159;  // 0.01 us of one of 148 SMs
+  const long long cost = sp_div(members + a.members - 1, a.members) * (1100 + 215 * tiles);
+  return saved > cost || a.always ? pages : 0;
 }
 
 // Tiles of a piece, chosen by one warp: each lane weighs one number of pieces of
@@ -261,16 +301,17 @@ __device__ __forceinline__ int sp_shared_pages(const SharedArgs& a, int given, i
 // own-keys kernel takes the SMs without a job at once and the others when
 // their jobs end.
 constexpr float kSpCostJob = 14.f, kSpCostTile = 2.2f, kSpCostOwn = 10.f;
-__device__ __forceinline__ int sp_choose_piece(const SharedArgs& a, const SpPlan& s, int longest, long long own_keys) {
+__device__ __forceinline__ int sp_choose_piece(const SharedArgs& a, const SpPlan& s, const SpDraft& d, int longest,
+                                              long long own_keys) {
   const int lane = threadIdx.x & 31, sms = gridDim.x;
   const int pieces = lane < 16 ? lane + 1 : 8 * lane - 104;  // 1 .. 16, 24, 32 .. 144
-  const int len = max(1, (longest + pieces - 1) / pieces);
+  const int len = max(1, sp_div(longest + pieces - 1, pieces));
   float jobs = 0.f;  // (their number can pass 31 bits before it is refused)
   for (int g = 0; g < a.groups; ++g)
     if (s.tiles[g] > 0)
-      jobs += (float)((s.cnt[g] + a.members - 1) / a.members * a.Hkv) * (float)((s.tiles[g] + len - 1) / len);
+      jobs += (float)(sp_div(d.cnt[g] + a.members - 1, a.members) * a.Hkv) * (float)sp_div(s.tiles[g] + len - 1, len);
   const float bytes = (float)own_keys * a.Hkv * 512.f;
-  const float shared = (kSpCostJob + kSpCostTile * len) * ceilf(jobs / sms);
+  const float shared = (kSpCostJob + kSpCostTile * len) * ceilf(__fdividef(jobs, (float)sms));
   const float rate = fminf(fmaxf(sms - jobs, 0.f) * 60e3f, 6.1e6f);     // bytes / us beside the jobs
   const float left = bytes - fmaxf(shared - kSpCostOwn, 0.f) * rate;     // when they end
   float cost = left > 0.f ? shared + 2.f + left / 6.1e6f : shared;
@@ -287,57 +328,38 @@ __device__ __forceinline__ int sp_choose_piece(const SharedArgs& a, const SpPlan
 __device__ __forceinline__ void sp_bar_tmem() { asm volatile("bar.sync 1, 288;" ::: "memory"); }
 
 // Builds the plan (every CTA the same) in shared memory.  All threads call it.
-__device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
+__device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s, SpDraft& d) {
   const int tid = threadIdx.x, lane = tid & 31;
-  auto row = [&](int b, int& nk) {  // group and keys of a row
-    nk = 0;
-    if (b >= a.B) return -1;
-    nk = a.cu_q[b + 1] > a.cu_q[b] ? max(a.cu_k[b + 1] - a.cu_k[b], 0) : 0;
-    return sp_group_of(a, b, blockIdx.x == 0);
-  };
-  int nk, g0 = row(tid, nk);  // (loaded beside the prefix lengths: one round trip)
-  for (int g = tid; g < a.groups; g += kSpThreads) {
-    s.cnt[g] = 0;
-    s.least[g] = 0x7fffffff;
-    s.tiles[g] = a.prefix_len[g];
-  }
-  if (tid == 0) s.keys = 0;
-  __syncthreads();
-  for (int b0 = 0; b0 < a.B; b0 += kSpThreads) {
-    const int b = b0 + tid;
-    if (b0 > 0) g0 = row(b, nk);
-    if (b < a.B) s.group[b] = (short)g0;
-    if (g0 >= 0) atomicMin(&s.least[g0], nk);
-    unsigned long long sum = nk;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) atomicAdd(&s.keys, sum);
-  }
-  __syncthreads();
-  if (tid < 32) {
-    // member numbers in batch order
+  for (int g = tid; g < a.groups; g += kSpThreads) s.tiles[g] = a.prefix_len[g];
+  sp_count_groups(a, d.cnt, d.least, &d.keys, d.group, kSpThreads);
+  // member numbers in batch order, by the last warp, beside the first one's work below
+  if (tid >= kSpThreads - 32) {
+    for (int g = lane; g < a.groups; g += 32) d.seen[g] = 0;
+    __syncwarp();
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       const int b = b0 + lane;
-      const int g = b < a.B ? s.group[b] : -1;
+      const int g = b < a.B ? d.group[b] : -1;
       const unsigned same = __match_any_sync(0xffffffffu, g);
       const int before = __popc(same & ((1u << lane) - 1u));
       int n = 0;
       if (g >= 0) {
-        n = s.cnt[g];
-        s.rank[b] = (short)(n + before);
+        n = d.seen[g];
+        d.rank[b] = (short)(n + before);
       }
       __syncwarp();
-      if (g >= 0 && before == 0) s.cnt[g] = n + __popc(same);
+      if (g >= 0 && before == 0) d.seen[g] = (short)(n + __popc(same));
       __syncwarp();
     }
+  }
+  if (tid < 32) {
     // prefixes, then the length of a piece, then first members and jobs
     int longest = 0;
     long long shared_keys = 0;
     for (int g = lane; g < a.groups; g += 32) {
-      const int tiles = sp_shared_pages(a, s.tiles[g], s.cnt[g], s.least[g]) * (a.page / kSpTile);
+      const int tiles = sp_shared_pages(a, s.tiles[g], d.cnt[g], d.least[g]) * (a.page / kSpTile);
       s.tiles[g] = tiles;
       longest = max(longest, tiles);
-      shared_keys += (long long)s.cnt[g] * tiles * kSpTile;
+      shared_keys += (long long)d.cnt[g] * tiles * kSpTile;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -345,15 +367,15 @@ __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
       shared_keys += __shfl_xor_sync(0xffffffffu, shared_keys, o);
     }
     __syncwarp();
-    const int len = sp_choose_piece(a, s, longest, (long long)s.keys - shared_keys);
+    const int len = sp_choose_piece(a, s, d, longest, (long long)d.keys - shared_keys);
     int members = 0, jobs = 0;
     for (int g0 = 0; g0 < a.groups; g0 += 32) {
       const int g = g0 + lane;
       int n = 0, split = 0, j = 0;
       if (g < a.groups) {
-        n = s.cnt[g];
-        split = (s.tiles[g] + len - 1) / len;
-        j = (n + a.members - 1) / a.members * a.Hkv * split;
+        n = d.cnt[g];
+        split = sp_div(s.tiles[g] + len - 1, len);
+        j = sp_div(n + a.members - 1, a.members) * a.Hkv * split;
       }
       int ni = n, ji = j;
 #pragma unroll
@@ -365,21 +387,21 @@ __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s) {
         }
       }
       if (g < a.groups) {
-        s.start[g] = members + ni - n;
+        s.start[g] = (short)(members + ni - n);
         s.off[g] = jobs + ji - j;
-        s.split[g] = split;
+        s.split[g] = (short)split;
       }
       members += __shfl_sync(0xffffffffu, ni, 31);
       jobs += __shfl_sync(0xffffffffu, ji, 31);
     }
     if (lane == 0) {
-      s.start[a.groups] = members;
+      s.start[a.groups] = (short)members;
       s.off[a.groups] = jobs;
     }
   }
   __syncthreads();
   for (int b = tid; b < a.B; b += kSpThreads)
-    if (s.group[b] >= 0) s.member[s.start[s.group[b]] + s.rank[b]] = (short)b;
+    if (d.group[b] >= 0) s.member[s.start[d.group[b]] + d.rank[b]] = (short)b;
   __syncthreads();
 }
 
@@ -398,12 +420,13 @@ __device__ __forceinline__ SpSeg sp_segment(const SharedArgs& a, const SpPlan& s
   }
   SpSeg g;
   g.g = lo;
-  const int n = s.start[lo + 1] - s.start[lo], split = s.split[lo];
-  const int blocks = (n + a.members - 1) / a.members;
-  const int at = (job - s.off[lo]) / split, piece = job - s.off[lo] - at * split;
-  g.k0 = (int)((long long)s.tiles[lo] * piece / split);
-  g.k1 = (int)((long long)s.tiles[lo] * (piece + 1) / split);
-  g.h = at / blocks;
+  const int n = s.start[lo + 1] - s.start[lo], split = s.split[lo], tiles = s.tiles[lo];
+  const int blocks = sp_div(n + a.members - 1, a.members);
+  const int at = sp_div(job - s.off[lo], split), piece = job - s.off[lo] - at * split;
+  const int each = sp_div(tiles, split), more = tiles - each * split;  // the first `more` pieces have one tile more
+  g.k0 = piece * each + min(piece, more);
+  g.k1 = g.k0 + each + (piece < more);
+  g.h = sp_div(at, blocks);
   g.block = at - g.h * blocks;
   g.rows = min(a.members, n - g.block * a.members) * a.G;
   g.nt = g.rows > 128 ? 2 : 1;
@@ -435,7 +458,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   uint64_t* drain = q_full + 10;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 11);
   volatile int* bad = reinterpret_cast<int*>(q_full + 12);  // some page is missing: the softmax looks which
-  SpPlan& plan = *reinterpret_cast<SpPlan*>(smem + kSpPlan);
+  SpPlan& plan = *reinterpret_cast<SpPlan*>(smem + kSpPlanAt);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -455,30 +478,34 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   }
   griddep_wait();
   griddep_launch_dependents();
-  sp_build_plan(a, plan);
+  SpDraft& draft = *reinterpret_cast<SpDraft*>(smem + kSpRing);
+  sp_build_plan(a, plan, draft);
   const int jobs = plan.off[a.groups];
-  if ((int)blockIdx.x >= jobs && blockIdx.x > 0) return;  // the whole CTA, before any TMEM
+  if (blockIdx.x == 0) {
+    // what the merge needs
+    for (int b = threadIdx.x; b < a.B; b += kSpThreads) {
+      SpRec r{};
+      const int g = draft.group[b];
+      if (g >= 0 && plan.tiles[g] > 0) {
+        r.keys = plan.tiles[g] * kSpTile;
+        r.split = plan.split[g];
+        r.off = plan.off[g];
+        r.start = plan.start[g];
+        r.members = plan.start[g + 1] - plan.start[g];
+        r.blocks = sp_div(r.members + a.members - 1, a.members);
+        r.rank = draft.rank[b];
+      }
+      a.rec[b] = r;
+    }
+  }
+  // the ring, with the draft in it, is the TMA's from here on
+  fence_proxy_async_smem();
+  __syncthreads();
+  if ((int)blockIdx.x >= jobs) return;  // the whole CTA, before any TMEM
   const uint32_t base = smem_u32(smem);
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSpRegsIssue));
-    // ---- what the merge needs
-    if (blockIdx.x == 0 && warp >= 2) {
-      for (int b = threadIdx.x - 64; b < a.B; b += 64) {
-        SpRec r{};
-        const int g = plan.group[b];
-        if (g >= 0 && plan.tiles[g] > 0) {
-          r.keys = plan.tiles[g] * kSpTile;
-          r.split = plan.split[g];
-          r.off = plan.off[g];
-          r.start = plan.start[g];
-          r.members = plan.start[g + 1] - plan.start[g];
-          r.blocks = (r.members + a.members - 1) / a.members;
-          r.rank = plan.rank[b];
-        }
-        a.rec[b] = r;
-      }
-    }
     // ---- producer
     if (warp == 0 && lane == 0) {
       int it = 0;      // loads issued; load it is in slot it % kSpSlots
@@ -567,7 +594,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         commit(&empty[it % kSpSlots]);
         for (int k = g.k0; k < g.k1; ++k, it += 2) {
           const bool more = k + 1 < g.k1;
-          ok = wait_slot(it + 1) && (!more || wait_slot(it + 2));
+          ok = wait_slot(it + 1);
           for (int t = 0; t < g.nt; ++t) {
             ok = ok && mbar_wait(&p_half[t], (uint32_t)step[t] & 1u, a.err);
             ok = __all_sync(0xffffffffu, ok);
@@ -581,6 +608,11 @@ __global__ void __launch_bounds__(kSpThreads, 1)
             tc_fence_after();
             values(t, it + 1, 1, true);
             // S_t's next scores overwrite P_t: MMAs of one thread run in the order of issue
+            if (more && t == 0) {
+              ok = wait_slot(it + 2);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+            }
             if (more) scores(t, it + 2);
             else commit(&o_done[t]);
           }

@@ -210,7 +210,7 @@ def test_shared_prefix_attention_refuses_before_any_launch():
                dict(rows=0), dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")), dict(scale=float("inf")),
                dict(q_stride=1028), dict(out=ctypes.c_void_p(264)), dict(k=ctypes.c_void_p(8)), dict(max_k=-1)):
         assert call(**kw) == -1, kw
-    for kw in (dict(Hq=18, Hkv=2), dict(B=1025), dict(groups=1025), dict(page=128), dict(Hq=65, Hkv=65),
+    for kw in (dict(Hq=18, Hkv=2), dict(B=1025), dict(groups=513), dict(page=128), dict(Hq=65, Hkv=65),
                dict(slots=1 << 31)):
         assert call(**kw) == -2, kw
 

@@ -17,9 +17,12 @@ DEV = "cuda"
 BF = torch.bfloat16
 
 
-@pytest.fixture(autouse=True)
-def _clean_error_word():
+@pytest.fixture(autouse=True, params=["", "always"])
+def _clean_error_word(request, monkeypatch):
+    """Every case twice: with the library's choice of the groups for which
+    sharing pays, and with every group of two or more sharing."""
     from src import b200
+    monkeypatch.setenv("B200_SHARED_PREFIX", request.param)
     b200.device_error(clear=True)
     yield
     assert b200.device_error(clear=True) == 0, "device error word set"
