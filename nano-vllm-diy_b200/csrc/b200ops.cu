@@ -1679,8 +1679,8 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   s.rest_o = reinterpret_cast<float*>(ws + l.rest_o);
   s.err = ds->err;
   // the shared part
-  if (int r = make_tmap_3d(&tmK, k_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kSpTile)) return r;
-  if (int r = make_tmap_3d(&tmV, v_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kSpTile)) return r;
+  if (int r = make_tmap_3d(&tmK, k_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kOwnTile)) return r;
+  if (int r = make_tmap_3d(&tmV, v_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kOwnTile)) return r;
   if (int r = check_prefix_registers()) return r;
   if (int r = ensure_smem(ds, 32u, shared_prefix_kernel, kSpSmemBytes)) return r;
   cudaError_t e = launch_ex(shared_prefix_kernel, dim3(ds->num_sms), dim3(kSpThreads), kSpSmemBytes, st, nullptr, 0,
@@ -1688,8 +1688,6 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
   if (int r = check_launch("shared_prefix_kernel")) return r;
   // every sequence's own keys
-  if (int r = make_tmap_3d(&tmK, k_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kOwnTile)) return r;
-  if (int r = make_tmap_3d(&tmV, v_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kOwnTile)) return r;
   if (int r = make_tmap_3d(&tmQ, q, kOwnHD, Hq, (uint64_t)num_q_rows, kOwnHD * 2, (uint64_t)q_stride * 2, 64,
                            (uint32_t)std::min(Hq, 8), 1))
     return r;

@@ -529,8 +529,12 @@ __global__ void __launch_bounds__(kSpThreads, 1)
             }
             const uint32_t dst = base + kSpRing + (uint32_t)sl * 32768u, bar = smem_u32(&full[sl]);
             mbar_arrive_expect_tx(&full[sl], 32768);
-            tma_load_3d(dst, kv ? &tmV : &tmK, bar, 0, g.h, (int)row);
-            tma_load_3d(dst + 16384, kv ? &tmV : &tmK, bar, 64, g.h, (int)row);
+            // (boxes of 32 keys: the tensor maps are those of the own keys)
+#pragma unroll
+            for (int r = 0; r < kSpTile; r += 32) {
+              tma_load_3d(dst + r * 128, kv ? &tmV : &tmK, bar, 0, g.h, (int)row + r);
+              tma_load_3d(dst + 16384 + r * 128, kv ? &tmV : &tmK, bar, 64, g.h, (int)row + r);
+            }
             ++it;
           }
         }

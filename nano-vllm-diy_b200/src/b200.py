@@ -13,7 +13,6 @@ and are reused by every call.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 
@@ -144,32 +143,45 @@ def _bf16(*ts: torch.Tensor | None) -> None:
             raise TypeError(f"expected bfloat16, got {t.dtype}")
 
 
-_SAME = contextlib.nullcontext()
+# the current stream's handle without the Stream object around it (several us a call)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _device_of(*ts: torch.Tensor | None):
-    """A context in which the current device (and so the current stream) is
-    that of the tensors, which must all be on one."""
+def _device_of(*ts: torch.Tensor | None) -> int:
+    """The device that holds the tensors; they must all be on one."""
     dev = None
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("b200 kernels need CUDA tensors (there is no CPU path)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return _SAME if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if t is not None:
+            d = t.get_device()
+            if d < 0:
+                raise RuntimeError("b200 kernels need CUDA tensors (there is no CPU path)")
+            if dev is None:
+                dev = d
+            elif d != dev:
+                raise ValueError(f"tensors on cuda:{dev} and cuda:{d}")
+    return dev
+
+
+def _call(name: str, dev: int, *args) -> None:
+    """lib.<name>(*args, stream) with `dev` as the current device and its current stream."""
+    fn = getattr(_lib or load_library(), name)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc != 0:
+        _check(rc, name)
 
 
 def _index(name: str, t: torch.Tensor, n: int | None = None) -> int:
     """Entries of an int32 vector the kernels index as t[i]."""
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32")
-    if t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1) or (n is not None and t.shape[0] != n):
+    shape = t.shape
+    if len(shape) != 1 or (n is not None and shape[0] != n) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous vector" + (f" of {n}" if n is not None else ""))
-    return t.shape[0]
+    return shape[0]
 
 
 def _rows(t: torch.Tensor) -> tuple[int, int]:
@@ -612,17 +624,24 @@ _prefix_ws_bytes: dict[tuple[int, ...], int] = {}
 
 def shared_prefix_workspace_bytes(max_seqs: int, max_seqlen_k: int, num_heads: int, num_kv_heads: int) -> int:
     """(of the current device: its size depends on the SM count)"""
-    key = (torch.cuda.current_device(), max_seqs, max_seqlen_k, num_heads, num_kv_heads)
+    size = ctypes.c_size_t(0)
+    _check(load_library().b200_shared_prefix_workspace_bytes(max_seqs, max_seqlen_k, num_heads, num_kv_heads,
+                                                             ctypes.byref(size)),
+           "b200_shared_prefix_workspace_bytes")
+    return int(size.value)
+
+
+def _prefix_workspace(dev: int, *shape: int) -> torch.Tensor:
+    key = (dev, *shape)
     n = _prefix_ws_bytes.get(key)
     if n is None:
-        size = ctypes.c_size_t(0)
-        _check(load_library().b200_shared_prefix_workspace_bytes(max_seqs, max_seqlen_k, num_heads,
-                                                                 num_kv_heads, ctypes.byref(size)),
-               "b200_shared_prefix_workspace_bytes")
-        if len(_prefix_ws_bytes) > 4096:
+        with torch.cuda.device(dev):
+            n = shared_prefix_workspace_bytes(*shape)
+        if len(_prefix_ws_bytes) >= 4096:
             _prefix_ws_bytes.clear()
-        n = _prefix_ws_bytes[key] = int(size.value)
-    return n
+        _prefix_ws_bytes[key] = n
+    buf = _workspaces.get((dev, "shared_prefix"))
+    return buf if buf is not None and buf.numel() >= n else workspace("shared_prefix", n, torch.device("cuda", dev))
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -635,35 +654,38 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     keys shared in each group, that is, the first prefix_len // page pages of the block tables of its
     sequences are the same (src.engine.metadata.shared_prefixes finds such groups).  The keys of a
     prefix are read once for its whole group."""
-    with _device_of(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, prefix_group, prefix_len, out):
-        _bf16(q, k_cache, v_cache, out)
-        B = _index("cu_seqlens_q", cu_seqlens_q) - 1
-        _index("cu_seqlens_k", cu_seqlens_k, B + 1)
-        _index("prefix_group", prefix_group, B)
-        groups = _index("prefix_len", prefix_len)
-        T, Hq, D = q.shape
-        if D != 128 or k_cache.dim() != 4 or k_cache.shape[3] != 128:
-            raise ValueError("head_dim must be 128 and the caches [pages, page, kv heads, 128]")
-        if v_cache.shape != k_cache.shape or not k_cache.is_contiguous() or not v_cache.is_contiguous():
-            raise ValueError("k_cache and v_cache must be contiguous and of one shape")
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
-            raise TypeError("block_table must be int32 [B, width] with contiguous rows")
-        if block_table.shape[0] != B:
-            raise ValueError(f"block_table of {block_table.shape[0]} rows for {B} sequences")
-        if q.stride(-1) != 1 or q.stride(1) != 128:
-            q = q.contiguous()
-        if out is None:
-            out = torch.empty(T, Hq, 128, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.stride(-1) != 1 or out.stride(1) != 128:
-            raise ValueError(f"out must be {tuple(q.shape)} with contiguous heads")
-        pages, page, Hkv, _ = k_cache.shape
-        ws = workspace("shared_prefix", shared_prefix_workspace_bytes(B, int(max_seqlen_k), Hq, Hkv), q.device)
-        _check(load_library().b200_shared_prefix_attention(
-            q.data_ptr(), q.stride(0), T, k_cache.data_ptr(), v_cache.data_ptr(), pages * page,
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cu_seqlens_q.data_ptr(),
-            cu_seqlens_k.data_ptr(), B, int(max_seqlen_k), Hq, Hkv, page, float(softmax_scale),
-            prefix_group.data_ptr(), prefix_len.data_ptr(), groups, out.data_ptr(), out.stride(0),
-            ws.data_ptr(), ws.numel(), _stream()), "b200_shared_prefix_attention")
+    dev = _device_of(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, prefix_group, prefix_len, out)
+    _bf16(q, k_cache, v_cache, out)
+    B = _index("cu_seqlens_q", cu_seqlens_q) - 1
+    _index("cu_seqlens_k", cu_seqlens_k, B + 1)
+    _index("prefix_group", prefix_group, B)
+    groups = _index("prefix_len", prefix_len)
+    T, Hq, D = q.shape
+    cache = k_cache.shape
+    if D != 128 or len(cache) != 4 or cache[3] != 128:
+        raise ValueError("head_dim must be 128 and the caches [pages, page, kv heads, 128]")
+    if v_cache.shape != cache or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise ValueError("k_cache and v_cache must be contiguous and of one shape")
+    table, stride = block_table.shape, block_table.stride()
+    if block_table.dtype is not torch.int32 or len(table) != 2 or stride[1] != 1:
+        raise TypeError("block_table must be int32 [B, width] with contiguous rows")
+    if table[0] != B:
+        raise ValueError(f"block_table of {table[0]} rows for {B} sequences")
+    q_stride = q.stride()
+    if q_stride[1:] != (128, 1):
+        q = q.contiguous()
+        q_stride = q.stride()
+    if out is None:
+        out = torch.empty((T, Hq, 128), dtype=torch.bfloat16, device=q.device)
+    elif out.shape != q.shape or out.stride()[1:] != (128, 1):
+        raise ValueError(f"out must be {tuple(q.shape)} with contiguous heads")
+    pages, page, Hkv, _ = cache
+    max_k = int(max_seqlen_k)
+    ws = _prefix_workspace(dev, B, max_k, Hq, Hkv)
+    _call("b200_shared_prefix_attention", dev, q.data_ptr(), q_stride[0], T, k_cache.data_ptr(), v_cache.data_ptr(),
+          pages * page, block_table.data_ptr(), stride[0], table[1], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+          B, max_k, Hq, Hkv, page, softmax_scale, prefix_group.data_ptr(), prefix_len.data_ptr(), groups,
+          out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel())
     return out
 
 
@@ -673,10 +695,10 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 def _cache_args(kv_cache: torch.Tensor):
     """C arguments of a cache [pages, page, Hkv, D] with up to two leading plane
     dimensions (the runner's [2, layers, pages, page, Hkv, D]) and contiguous pages."""
-    d = kv_cache.dim()
+    shape, stride, size = kv_cache.shape, kv_cache.stride(), kv_cache.element_size()
+    d = len(shape)
     if d < 4 or d > 6:
         raise ValueError("kv_cache must be [pages, page, heads, dim], with up to two leading dimensions")
-    shape, stride, size = kv_cache.shape, kv_cache.stride(), kv_cache.element_size()
     pages, page, heads, dim = shape[-4:]
     if stride[-1] != 1 or stride[-2] != dim or stride[-3] != heads * dim:
         raise ValueError("kv_cache: the slots of a page must be contiguous")
@@ -686,15 +708,16 @@ def _cache_args(kv_cache: torch.Tensor):
 
 
 def _table_args(block_tables: torch.Tensor, seq_lens: torch.Tensor | None, refs: torch.Tensor):
-    if block_tables.dtype != torch.int32:
+    if block_tables.dtype is not torch.int32:
         raise TypeError("block_tables must be int32")
-    if block_tables.dim() != 2 or block_tables.stride(1) != 1:
+    shape, stride = block_tables.shape, block_tables.stride()
+    if len(shape) != 2 or stride[1] != 1:
         raise ValueError("block_tables must be [rows, width] with contiguous rows")
-    rows, width = block_tables.shape
+    rows, width = shape
     if seq_lens is not None:
         _index("seq_lens", seq_lens, rows)
     _index("refs", refs)
-    return block_tables.data_ptr(), block_tables.stride(0) if rows > 1 else width, rows, width
+    return block_tables.data_ptr(), stride[0] if rows > 1 else width, rows, width
 
 
 def copy_pages(kv_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -702,13 +725,13 @@ def copy_pages(kv_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
     """kv_cache[..., dst[i], :num_tokens[i]] = kv_cache[..., src[i], :num_tokens[i]] in every plane
     (whole pages without num_tokens).  int32 indices on the device, -1 skips; no page may be the
     destination of two copies, or the source of one and the destination of another."""
-    with _device_of(kv_cache, src, dst, num_tokens):
-        n = _index("src", src)
-        _index("dst", dst, n)
-        if num_tokens is not None:
-            _index("num_tokens", num_tokens, n)
-        _check(load_library().b200_copy_pages(*_cache_args(kv_cache), _p(src), _p(dst), _p(num_tokens), n,
-                                              _stream()), "b200_copy_pages")
+    dev = _device_of(kv_cache, src, dst, num_tokens)
+    n = _index("src", src)
+    _index("dst", dst, n)
+    if num_tokens is not None:
+        _index("num_tokens", num_tokens, n)
+    _call("b200_copy_pages", dev, *_cache_args(kv_cache), src.data_ptr(), dst.data_ptr(),
+          None if num_tokens is None else num_tokens.data_ptr(), n)
 
 
 def take_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor,
@@ -716,23 +739,22 @@ def take_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.T
     """The rows grow to new_lens tokens and get the pages they lack, lowest free ones first in the
     order of the list.  Returns int32 done [n]: 0 where a row stays as it was (it would shrink or
     outgrow its table, is listed before, or the list up to it needs more pages than are free)."""
-    with _device_of(block_tables, seq_lens, refs, rows, new_lens):
-        n = _index("rows", rows)
-        _index("new_lens", new_lens, n)
-        tables = _table_args(block_tables, seq_lens, refs)
-        done = torch.empty_like(rows)
-        _check(load_library().b200_take_pages(*tables, _p(seq_lens), _p(refs), refs.shape[0], int(page), _p(rows),
-                                              _p(new_lens), n, _p(done), _stream()), "b200_take_pages")
+    dev = _device_of(block_tables, seq_lens, refs, rows, new_lens)
+    n = _index("rows", rows)
+    _index("new_lens", new_lens, n)
+    tables = _table_args(block_tables, seq_lens, refs)
+    done = torch.empty_like(rows)
+    _call("b200_take_pages", dev, *tables, seq_lens.data_ptr(), refs.data_ptr(), refs.shape[0], int(page),
+          rows.data_ptr(), new_lens.data_ptr(), n, done.data_ptr())
     return done
 
 
 def free_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor) -> None:
     """The rows give their pages back (one reference less for each) and are empty afterwards."""
-    with _device_of(block_tables, seq_lens, refs, rows):
-        n = _index("rows", rows)
-        tables = _table_args(block_tables, seq_lens, refs)
-        _check(load_library().b200_free_pages(*tables, _p(seq_lens), _p(refs), refs.shape[0], _p(rows), n,
-                                              _stream()), "b200_free_pages")
+    dev = _device_of(block_tables, seq_lens, refs, rows)
+    n = _index("rows", rows)
+    tables = _table_args(block_tables, seq_lens, refs)
+    _call("b200_free_pages", dev, *tables, seq_lens.data_ptr(), refs.data_ptr(), refs.shape[0], rows.data_ptr(), n)
 
 
 def fork_pages(kv_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor,
@@ -740,36 +762,36 @@ def fork_pages(kv_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: tor
     """Row children[i] (empty) becomes a fork of row parents[i]: the parent's full pages shared, the
     used part of a last page that is not full copied to the lowest free page.  Returns int32 done
     [n]: 0 where nothing changed (the child is not empty or listed before, or no page is left)."""
-    with _device_of(kv_cache, block_tables, seq_lens, refs, parents, children):
-        n = _index("parents", parents)
-        _index("children", children, n)
-        cache = _cache_args(kv_cache)
-        tables = _table_args(block_tables, seq_lens, refs)
-        if refs.shape[0] != cache[6]:
-            raise ValueError(f"refs of {refs.shape[0]} pages for a cache of {cache[6]}")
-        # plan and result in one allocation: [n][4] words of scratch, then done
-        out = torch.empty(5 * n, dtype=torch.int32, device=parents.device)
-        done = out[4 * n:]
-        _check(load_library().b200_fork_pages(*cache, *tables, _p(seq_lens), _p(refs), _p(parents), _p(children), n,
-                                              _p(out), _p(done), _stream()), "b200_fork_pages")
-    return done
+    dev = _device_of(kv_cache, block_tables, seq_lens, refs, parents, children)
+    n = _index("parents", parents)
+    _index("children", children, n)
+    cache = _cache_args(kv_cache)
+    tables = _table_args(block_tables, seq_lens, refs)
+    if refs.shape[0] != cache[6]:
+        raise ValueError(f"refs of {refs.shape[0]} pages for a cache of {cache[6]}")
+    # result and plan in one allocation: done, then (16-byte aligned) [n][4] words of scratch
+    at = (n + 3) // 4 * 4
+    out = torch.empty(at + 4 * n, dtype=torch.int32, device=parents.device)
+    ptr = out.data_ptr()
+    _call("b200_fork_pages", dev, *cache, *tables, seq_lens.data_ptr(), refs.data_ptr(), parents.data_ptr(),
+          children.data_ptr(), n, ptr + 4 * at, ptr)
+    return out[:n]
 
 
 def compact_pages(kv_cache: torch.Tensor, block_tables: torch.Tensor, refs: torch.Tensor) -> torch.Tensor:
     """Moves the N live pages (refs != 0) into pages [0, N): the k-th live page behind them into the
     k-th free one among them; tables and refs follow.  Returns int32 place [pages]: where each
     page's contents are now, -1 for a free page."""
-    with _device_of(kv_cache, block_tables, refs):
-        cache = _cache_args(kv_cache)
-        tables = _table_args(block_tables, None, refs)
-        pages = cache[6]
-        if refs.shape[0] != pages:
-            raise ValueError(f"refs of {refs.shape[0]} pages for a cache of {pages}")
-        place = torch.empty_like(refs)
-        moves = torch.empty(2 + pages, dtype=torch.int32, device=refs.device)
-        _check(load_library().b200_compact_pages(*cache, *tables, _p(refs), _p(place), _p(moves), _stream()),
-               "b200_compact_pages")
-    return place
+    dev = _device_of(kv_cache, block_tables, refs)
+    cache = _cache_args(kv_cache)
+    tables = _table_args(block_tables, None, refs)
+    pages = cache[6]
+    if refs.shape[0] != pages:
+        raise ValueError(f"refs of {refs.shape[0]} pages for a cache of {pages}")
+    out = torch.empty(2 * pages + 2, dtype=torch.int32, device=refs.device)  # result, then scratch
+    ptr = out.data_ptr()
+    _call("b200_compact_pages", dev, *cache, *tables, refs.data_ptr(), ptr, ptr + 4 * pages)
+    return out[:pages]
 
 
 # ---------------------------------------------------------------------------
