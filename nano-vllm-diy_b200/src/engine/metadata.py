@@ -144,3 +144,61 @@ def build_on_device(seqs, block_size: int, device) -> tuple[torch.Tensor, torch.
                       if attends_cache else None),
     )
     return ids_dev, positions, ctx
+
+
+def shared_prefixes(tables: list[list[int]], lens: list[int], block_size: int) -> tuple[np.ndarray, np.ndarray]:
+    """Groups of sequences whose block tables begin with the same blocks:
+    (int32 [B] group of each sequence or -1, int32 [groups] shared keys), for
+    b200.shared_prefix_attention.  The blocks are those that the reference's
+    prefix cache shares (src/engine/block_manager.py:96-181) or that forks have
+    in common.  `lens`: keys of each sequence; only full blocks count.
+
+    Sequences can share prefixes of different lengths (all a system prompt,
+    some a document behind it) but belong to one group each.  Sorted by table,
+    the runs of neighbours with a common prefix nest; from the innermost run
+    outwards, the sequences in no group yet form one with the blocks common to
+    the run, and an inner group joins them where that saves more block reads.
+    """
+    B = len(tables)
+    group = np.full(B, -1, dtype=np.int32)
+    order = sorted(range(B), key=lambda b: tables[b])
+    full = [min(len(tables[b]), lens[b] // block_size) for b in order]
+    # common full blocks of neighbours in the sorted order
+    common = []
+    for i in range(1, B):
+        x, y = tables[order[i - 1]], tables[order[i]]
+        n = min(full[i - 1], full[i])
+        k = 0
+        while k < n and x[k] == y[k]:
+            k += 1
+        common.append(k)
+    # open runs, inner ones on top: [blocks in common, rows in no group, groups (rows, blocks)]
+    runs: list[list] = []
+    closed: list[tuple[list[int], int]] = []
+    for i, k in enumerate(common + [0]):
+        rest, groups = [i], []
+        while runs and runs[-1][0] >= k:
+            depth, r, g = runs.pop()
+            rest, groups = _close_run(depth, r + rest, g + groups)
+        if k > 0:
+            runs.append([k, rest, groups])
+        else:
+            closed += groups
+    for g, (rows, depth) in enumerate(closed):
+        group[[order[j] for j in rows]] = g
+    lens_out = [depth * block_size for _, depth in closed]
+    return group, np.asarray(lens_out, dtype=np.int32)
+
+
+def _close_run(depth: int, rest: list[int], groups: list) -> tuple[list[int], list]:
+    """The rows of a run with `depth` blocks in common: `rest` in no group yet
+    and inner groups (rows, blocks).  A group of s rows saves s - 1 times its
+    blocks; its rows in an outer group that has others save s times `depth`."""
+    join = [g for g in groups if len(g[0]) * depth > (len(g[0]) - 1) * g[1]]
+    gain = sum(len(g[0]) * depth - (len(g[0]) - 1) * g[1] for g in join)
+    if join and (rest or gain > depth):
+        groups = [g for g in groups if g not in join]
+        rest = rest + [row for g in join for row in g[0]]
+    if len(rest) >= 2:
+        return [], groups + [(rest, depth)]
+    return rest, groups

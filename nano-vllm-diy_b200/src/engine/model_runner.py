@@ -23,6 +23,7 @@ import torch
 
 from src import b200
 from src.engine import metadata as M
+from src.engine.pages import PagePool
 from src.models.qwen3 import Qwen3ForCausalLM
 from src.utils.context import Context
 from src.utils.loader import load_weights
@@ -32,7 +33,10 @@ class ModelRunner:
 
     def __init__(self, config, rank: int = 0, world_size: int = 1, block_size: int = 256,
                  max_num_seqs: int = 256, max_seq_len: int = 8192, enforce_eager: bool = False,
-                 device: torch.device | None = None):
+                 device: torch.device | None = None, shared_prefix: bool = False):
+        """shared_prefix: decode steps find the sequences whose block tables
+        begin with the same blocks and attend over those once for all of them
+        (b200.shared_prefix_attention)."""
         self.config = config
         self.rank = rank
         self.world_size = world_size
@@ -40,6 +44,7 @@ class ModelRunner:
         self.max_num_seqs = max_num_seqs
         self.max_seq_len = max_seq_len
         self.enforce_eager = enforce_eager
+        self.shared_prefix = shared_prefix
         self.device = device or torch.device("cuda", torch.cuda.current_device())
         prev_dtype = torch.get_default_dtype()
         prev_device = torch.get_default_device()
@@ -93,6 +98,15 @@ class ModelRunner:
         self.num_kvcache_blocks = num_blocks
         nbytes = b200.attention_workspace_bytes(self.max_num_seqs, self.max_seq_len, self.local_q_heads)
         b200.reserve_workspace("attn", nbytes, self.device)
+        if self.shared_prefix:
+            nbytes = b200.shared_prefix_workspace_bytes(self.max_num_seqs, self.max_seq_len, self.local_q_heads,
+                                                        self.local_kv_heads)
+            b200.reserve_workspace("shared_prefix", nbytes, self.device)
+
+    def page_pool(self, max_rows: int | None = None) -> PagePool:
+        """A pool over this runner's cache, whose tables live on the device (the
+        block tables of sequences passed to prepare() must then not be used)."""
+        return PagePool(self.kv_cache, max_rows or self.max_num_seqs, self.max_seq_len)
 
     # ------------------------------------------------------------------ steps
     def prepare(self, seqs) -> tuple[torch.Tensor, torch.Tensor, Context]:
@@ -101,8 +115,16 @@ class ModelRunner:
         (b200_step_metadata); B200_HOST_METADATA=1 builds everything on the
         host instead."""
         if os.environ.get("B200_HOST_METADATA") == "1":
-            return M.to_device(M.build(seqs, self.block_size), self.device)
-        return M.build_on_device(seqs, self.block_size, self.device)
+            step = M.to_device(M.build(seqs, self.block_size), self.device)
+        else:
+            step = M.build_on_device(seqs, self.block_size, self.device)
+        ctx = step[2]
+        if self.shared_prefix and ctx.max_seqlen_q == 1 and ctx.block_tables is not None:
+            lens = [min(s.num_cached_tokens, len(s) - 1) + s.num_scheduled_tokens for s in seqs]
+            group, prefix = M.shared_prefixes([s.block_table for s in seqs], lens, self.block_size)
+            ctx.prefix_group, ctx.prefix_lens = (torch.from_numpy(a).pin_memory().to(self.device, non_blocking=True)
+                                                 for a in (group, prefix))
+        return step
 
     @torch.inference_mode()
     def run_hidden(self, input_ids: torch.Tensor, positions: torch.Tensor,
@@ -124,6 +146,11 @@ class ModelRunner:
         v["cu_seqlens_k"][:bs + 1] = ctx.cu_seqlens_k
         v["block_tables"].fill_(-1)
         v["block_tables"][:bs, :ctx.block_tables.size(1)] = ctx.block_tables
+        if self.shared_prefix:
+            v["prefix_group"].fill_(-1)
+            if ctx.prefix_group is not None:
+                v["prefix_group"][:bs] = ctx.prefix_group
+                v["prefix_lens"][:ctx.prefix_lens.size(0)] = ctx.prefix_lens
         self.graphs[gbs].replay()
         return v["outputs"][:bs], Context(is_prefill=False)
 
@@ -173,6 +200,10 @@ class ModelRunner:
             outputs=torch.zeros(max_bs, self.config.hidden_size, dtype=torch.bfloat16, device=dev),
             tokens=torch.zeros(max_bs, dtype=torch.int64, device=dev),
         )
+        if self.shared_prefix:
+            # groups of two at least; a sequence in none has -1
+            v["prefix_group"] = torch.full((max_bs,), -1, dtype=torch.int32, device=dev)
+            v["prefix_lens"] = torch.zeros(max(max_bs // 2, 1), dtype=torch.int32, device=dev)
         self.graph_with_sampling = with_sampling
         self.graph_vars = v
         for bs in sorted(batch_sizes, reverse=True):
@@ -180,6 +211,9 @@ class ModelRunner:
                           cu_seqlens_k=v["cu_seqlens_k"][:bs + 1], max_seqlen_q=1,
                           max_seqlen_k=self.max_seq_len, slot_mapping=v["slot_mapping"][:bs],
                           block_tables=v["block_tables"][:bs])
+            if self.shared_prefix:
+                ctx.prefix_group = v["prefix_group"][:bs]
+                ctx.prefix_lens = v["prefix_lens"][:max(bs // 2, 1)]
             def step():
                 v["outputs"][:bs] = self.model(v["input_ids"][:bs], v["positions"][:bs], ctx)
                 if with_sampling:

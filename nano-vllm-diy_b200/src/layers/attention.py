@@ -7,7 +7,9 @@ slot -1.  Attention.forward(q, k, v, ctx) scatters when the cache is
 allocated, then attends causally (bottom-right aligned) with GQA, reading K/V
 from the paged cache through ctx.block_tables when they are set and from the
 per-token k / v otherwise -- flash_attn_varlen_func's contract at
-attention.py:93-104, on the sm_100a kernels.
+attention.py:93-104, on the sm_100a kernels.  A decode batch whose context
+names groups of sequences with a common prefix reads each prefix once for its
+group.
 """
 from __future__ import annotations
 
@@ -29,6 +31,10 @@ def attend(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
            k_cache: torch.Tensor, v_cache: torch.Tensor, ctx: Context, scale: float,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over the batch described by ctx (no cache write)."""
+    if ctx.prefix_group is not None and ctx.block_tables is not None and ctx.max_seqlen_q == 1:
+        return b200.shared_prefix_attention(q, k_cache, v_cache, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
+                                            ctx.max_seqlen_k, scale, ctx.block_tables, ctx.prefix_group,
+                                            ctx.prefix_lens, out=out)
     if ctx.block_tables is not None:
         return b200.paged_attention(q, None, None, k_cache, v_cache, ctx.cu_seqlens_q,
                                     ctx.cu_seqlens_k, ctx.max_seqlen_q, ctx.max_seqlen_k, scale,

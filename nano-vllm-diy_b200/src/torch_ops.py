@@ -130,6 +130,80 @@ def _(q, k, v, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_s
     return q.new_empty(q.shape)
 
 
+@_op("shared_prefix_attention")
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, max_seqlen_k: int,
+                            softmax_scale: float, block_table: torch.Tensor, prefix_group: torch.Tensor,
+                            prefix_len: torch.Tensor) -> torch.Tensor:
+    """paged_attention of a decode batch, the keys of shared prefixes read once."""
+    return b200.shared_prefix_attention(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_k,
+                                        softmax_scale, block_table, prefix_group, prefix_len)
+
+
+@shared_prefix_attention.register_fake
+def _(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_k, softmax_scale, block_table, prefix_group,
+      prefix_len):
+    return q.new_empty(q.shape)
+
+
+@_op("copy_pages", mutates=("kv_cache",))
+def copy_pages(kv_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+               num_tokens: Optional[torch.Tensor] = None) -> None:
+    """Pages dst[i] := src[i], their first num_tokens[i] slots."""
+    b200.copy_pages(kv_cache, src, dst, num_tokens)
+
+
+@copy_pages.register_fake
+def _(kv_cache, src, dst, num_tokens=None):
+    return None
+
+
+@_op("take_pages", mutates=("block_tables", "seq_lens", "refs"))
+def take_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor,
+               new_lens: torch.Tensor, page: int) -> torch.Tensor:
+    """Rows grow to new_lens tokens; int32 done."""
+    return b200.take_pages(block_tables, seq_lens, refs, rows, new_lens, page)
+
+
+@take_pages.register_fake
+def _(block_tables, seq_lens, refs, rows, new_lens, page):
+    return rows.new_empty(rows.shape)
+
+
+@_op("free_pages", mutates=("block_tables", "seq_lens", "refs"))
+def free_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor) -> None:
+    """Rows give their pages back."""
+    b200.free_pages(block_tables, seq_lens, refs, rows)
+
+
+@free_pages.register_fake
+def _(block_tables, seq_lens, refs, rows):
+    return None
+
+
+@_op("fork_pages", mutates=("kv_cache", "block_tables", "seq_lens", "refs"))
+def fork_pages(kv_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor,
+               parents: torch.Tensor, children: torch.Tensor) -> torch.Tensor:
+    """Rows children become forks of rows parents; int32 done."""
+    return b200.fork_pages(kv_cache, block_tables, seq_lens, refs, parents, children)
+
+
+@fork_pages.register_fake
+def _(kv_cache, block_tables, seq_lens, refs, parents, children):
+    return parents.new_empty(parents.shape)
+
+
+@_op("compact_pages", mutates=("kv_cache", "block_tables", "refs"))
+def compact_pages(kv_cache: torch.Tensor, block_tables: torch.Tensor, refs: torch.Tensor) -> torch.Tensor:
+    """Live pages to the front; int32 place of every page."""
+    return b200.compact_pages(kv_cache, block_tables, refs)
+
+
+@compact_pages.register_fake
+def _(kv_cache, block_tables, refs):
+    return refs.new_empty(refs.shape)
+
+
 @_op("embedding")
 def embedding(ids: torch.Tensor, weight: torch.Tensor, vocab_start: int, vocab_end: int) -> torch.Tensor:
     """VocabParallelEmbedding's masked lookup (src/layers/llm_head.py:38-47)."""
@@ -153,4 +227,5 @@ def _(logits):
 
 
 OPS = ("linear", "linear_silu_and_mul", "rms_norm", "rms_norm_residual", "silu_and_mul", "store_kvcache",
-       "qk_norm_rope_store", "paged_attention", "embedding", "argmax")
+       "qk_norm_rope_store", "paged_attention", "shared_prefix_attention", "copy_pages", "take_pages", "free_pages",
+       "fork_pages", "compact_pages", "embedding", "argmax")

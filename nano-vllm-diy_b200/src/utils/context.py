@@ -1,6 +1,7 @@
 """Per-step attention metadata, the same record as the reference's
 src/utils/context.py:5-14 (field names, order and defaults are part of the
-interface that ModelRunner fills in and the layers read)."""
+interface that ModelRunner fills in and the layers read), and behind its
+fields the groups of sequences that share a prefix, for decode batches."""
 from dataclasses import dataclass
 
 from torch import Tensor
@@ -16,3 +17,5 @@ class Context:
     slot_mapping: Tensor | None = None      # int32 [T], -1 = no cache write
     context_lens: Tensor | None = None      # int32 [B]
     block_tables: Tensor | None = None      # int32 [B, max_blocks], -1 padded
+    prefix_group: Tensor | None = None      # int32 [B], group of each sequence or -1
+    prefix_lens: Tensor | None = None       # int32 [groups], keys shared in each group
