@@ -1746,14 +1746,6 @@ int page_tables(const char* what, int* block_tables, long long bt_stride, int ro
   return B200_OK;
 }
 
-// One resident wave of content CTAs (4 of 256 threads on each SM keep 128 KB
-// of loads in flight), or one CTA per unit when there are fewer.
-int page_grid(long long units) {
-  DeviceState* ds;
-  if (device_state(&ds)) return 1;
-  return (int)std::max<long long>(1, std::min<long long>(units, (long long)ds->num_sms * 4));
-}
-
 }  // namespace
 
 extern "C" int b200_copy_pages(void* cache, long long s0, long long s1, long long page_stride, int n0, int n1,
@@ -1766,7 +1758,7 @@ extern "C" int b200_copy_pages(void* cache, long long s0, long long s1, long lon
   DeviceState* ds;
   if (int r = device_state(&ds)) return r;
   const long long units = (long long)n * c.planes * ((c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs);
-  launch_ex(copy_pages_kernel, dim3(page_grid(units)), dim3(kPgThreads), 0, reinterpret_cast<cudaStream_t>(stream),
+  launch_ex(copy_pages_kernel, dim3((unsigned)std::min<long long>(units, kPgGrid)), dim3(kPgThreads), 0, reinterpret_cast<cudaStream_t>(stream),
             nullptr, 0, c, src, dst, num_tokens, n, num_pages, page, ds->err);
   return check_launch("copy_pages_kernel");
 }
@@ -1814,8 +1806,8 @@ extern "C" int b200_fork_pages(void* cache, long long s0, long long s1, long lon
   launch_ex(fork_plan_kernel, dim3(1), dim3(kPgMax), 0, st, nullptr, 0, t, parents, children, n, plan, done);
   if (int r = check_launch("fork_plan_kernel")) return r;
   const long long units = n + (long long)n * c.planes * ((c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs);
-  launch_ex(fork_apply_kernel, dim3(page_grid(units)), dim3(kPgThreads), 0, st, nullptr, 0, t, c, parents, children,
-            n, static_cast<const int*>(plan));
+  launch_overlapped(fork_apply_kernel, (int)std::min<long long>(units, kPgGrid), kPgThreads, 0, st, t, c, parents,
+                    children, n, static_cast<const int*>(plan));
   return check_launch("fork_apply_kernel");
 }
 
@@ -1835,7 +1827,7 @@ extern "C" int b200_compact_pages(void* cache, long long s0, long long s1, long 
   if (int r = check_launch("compact_plan_kernel")) return r;
   const long long pieces = (c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs;
   const long long units = ((long long)rows * width + kPgThreads - 1) / kPgThreads + num_pages / 2 * c.planes * pieces;
-  launch_ex(compact_apply_kernel, dim3(page_grid(units)), dim3(kPgThreads), 0, st, nullptr, 0, t, c,
-            static_cast<const int*>(place), static_cast<const int*>(moves));
+  launch_overlapped(compact_apply_kernel, (int)std::min<long long>(units, kPgGridUnknown), kPgThreads, 0, st, t, c,
+                    static_cast<const int*>(place), static_cast<const int*>(moves));
   return check_launch("compact_apply_kernel");
 }

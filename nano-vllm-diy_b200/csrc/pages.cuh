@@ -13,8 +13,12 @@
 //     its first rank, and a second walk hands page k of the free list to the
 //     request whose prefix sum of needs covers k (a binary search in shared
 //     memory).  No order depends on a race, so results are the same every time.
-//   * contents: HBM-bound copies of page heads over all planes, in pieces of
-//     kPgPiece bytes over the whole grid.
+//   * contents: HBM-bound copies of page heads over all planes in pieces of 32 KB,
+//     one CTA each, handed out by the hardware: 6.41 TB/s with 24 ragged page
+//     pairs of 72 planes, 6.53 with whole pages (99 % of a plain copy), where a
+//     resident grid that strides over the pieces stayed at 4.9 to 5.9 and bulk
+//     copies through shared memory at 5.7: pieces that start together then lie
+//     together.  More than kPgGrid pieces share the CTAs (measured: within 1 %).
 // A fork or a compaction is a decision launch and a content launch, in stream
 // order; what the second needs lies in a plan array of the caller's.
 #pragma once
@@ -26,6 +30,8 @@ constexpr int kPgMax = 1024;            // requests of one call: one thread each
 constexpr int kPgHash = 4 * kPgMax;     // slots of the table that finds repeated rows
 constexpr int kPgThreads = 256;         // content kernels
 constexpr int kPgPieceVecs = 2048;      // 16-byte vectors of one piece (32 KB: 8 a thread, all in flight)
+constexpr int kPgGrid = 16384;          // CTAs of a content launch
+constexpr int kPgGridUnknown = 8192;    // where only the device knows how many have work (empty ones: 6 us)
 constexpr int kPgPlanWords = 4;         // fork plan: {source page, fresh page, tokens of the last page, full pages (-1: no fork)}
 
 struct PageTables {
@@ -89,18 +95,43 @@ __device__ __forceinline__ int4 pg_refs4(const int* refs, int p, int end) {
   return v;
 }
 
-__device__ __forceinline__ int pg_count_free(const int* refs, int beg, int end) {
-  int n = 0;
-  for (int p = beg; p < end; p += 4) {
-    const int4 v = pg_refs4(refs, p, end);
-    n += (v.x == 0) + (v.y == 0) + (v.z == 0) + (v.w == 0);
+// The free pages of a stretch: as bits where 64 cover it, else read again for
+// each walk.
+struct PgFree {
+  int beg, end;
+  unsigned long long bits;
+  int count;
+};
+__device__ __forceinline__ PgFree pg_free_pages(const int* refs, int pages) {
+  PgFree f;
+  pg_stretch(pages, f.beg, f.end);
+  f.bits = 0;
+  f.count = 0;
+  const bool few = f.end - f.beg <= 64;
+  for (int p = f.beg; p < f.end; p += 4) {
+    const int4 v = pg_refs4(refs, p, f.end);
+    const unsigned m = (v.x == 0) | (v.y == 0) << 1 | (v.z == 0) << 2 | (v.w == 0) << 3;
+    f.count += __popc(m);
+    if (few) f.bits |= (unsigned long long)m << (p - f.beg);
   }
-  return n;
+  return f;
+}
+// take(rank, page) for the free pages of the stretch, the first of which has
+// rank `rank`, as far as ranks below `asked` go.
+template <typename F>
+__device__ __forceinline__ void pg_walk(const PgFree& f, const int* refs, int rank, int asked, F take) {
+  if (f.end - f.beg <= 64) {
+    for (unsigned long long m = f.bits; m != 0 && rank < asked; m &= m - 1) take(rank++, f.beg + __ffsll(m) - 1);
+    return;
+  }
+  for (int p = f.beg; p < f.end && rank < asked; ++p)
+    if (refs[p] == 0) take(rank++, p);
 }
 
-// First index t with incl[t] > k (incl ascending, n entries, incl[n - 1] > k).
-__device__ __forceinline__ int pg_owner(const int* incl, int n, int k) {
-  int lo = 0, hi = n - 1;
+// First index t from `lo` on with incl[t] > k (incl ascending, n entries, incl[n - 1] > k).
+__device__ __forceinline__ int pg_owner(const int* incl, int n, int k, int lo) {
+  if (incl[lo] > k) return lo;
+  int hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (incl[mid] > k) hi = mid; else lo = mid + 1;
@@ -166,13 +197,11 @@ __global__ void __launch_bounds__(kPgMax, 1)
     ok = len >= 0 && want >= len && to <= a.width;
     need = ok ? to - held : 0;
   }
-  int beg, end, asked, free_pages, dummy;
+  int asked, free_pages;
+  const PgFree f = pg_free_pages(a.refs, a.pages);
   const int incl = pg_scan(need, s.sums, asked);
   s.incl[t] = incl;
-  pg_stretch(a.pages, beg, end);
-  const int mine = pg_count_free(a.refs, beg, end);
-  int rank = pg_scan(mine, s.sums, free_pages) - mine;
-  (void)dummy;
+  const int rank = pg_scan(f.count, s.sums, free_pages) - f.count;
   // a row is served when the needs up to and with its own fit the free pages
   const bool done = ok && (need == 0 || incl <= free_pages);
   if (t < n) done_out[t] = done;
@@ -181,22 +210,13 @@ __global__ void __launch_bounds__(kPgMax, 1)
   s.first[t] = held - (incl - need);
   if (done) a.lens[row] = want;
   __syncthreads();
-  for (int p = beg; p < end && rank < asked; p += 4) {
-    const int4 v = pg_refs4(a.refs, p, end);
-    const int r[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (r[i] != 0) continue;
-      if (rank < asked) {
-        const int o = pg_owner(s.incl, kPgMax, rank);
-        if (s.keys[o] >= 0) {
-          a.tables[(long long)s.keys[o] * a.stride + s.first[o] + rank] = p + i;
-          a.refs[p + i] = 1;
-        }
-      }
-      ++rank;
-    }
-  }
+  int o = 0;
+  pg_walk(f, a.refs, rank, asked, [&](int k, int p) {
+    o = pg_owner(s.incl, kPgMax, k, o);
+    if (s.keys[o] < 0) return;
+    a.tables[(long long)s.keys[o] * a.stride + s.first[o] + k] = p;
+    a.refs[p] = 1;
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -270,12 +290,11 @@ __global__ void __launch_bounds__(kPgMax, 1)
     }
   }
   const int need = ok && part > 0;
-  int beg, end, asked, free_pages;
+  int asked, free_pages;
+  const PgFree f = pg_free_pages(a.refs, a.pages);
   const int incl = pg_scan(need, s.sums, asked);
   s.incl[t] = incl;
-  pg_stretch(a.pages, beg, end);
-  const int mine = pg_count_free(a.refs, beg, end);
-  int rank = pg_scan(mine, s.sums, free_pages) - mine;
+  const int rank = pg_scan(f.count, s.sums, free_pages) - f.count;
   const bool done = ok && (!need || incl <= free_pages);
   if (t < n) {
     done_out[t] = done;
@@ -286,38 +305,28 @@ __global__ void __launch_bounds__(kPgMax, 1)
   if (done) a.lens[child] = len;
   s.keys[t] = done && need;
   __syncthreads();
-  for (int p = beg; p < end && rank < asked; p += 4) {
-    const int4 v = pg_refs4(a.refs, p, end);
-    const int r[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (r[i] != 0) continue;
-      if (rank < asked) {
-        const int o = pg_owner(s.incl, kPgMax, rank);
-        if (s.keys[o]) {
-          plan[o * kPgPlanWords + 1] = p + i;
-          a.refs[p + i] = 1;
-        }
-      }
-      ++rank;
-    }
-  }
+  int o = 0;
+  pg_walk(f, a.refs, rank, asked, [&](int k, int p) {
+    o = pg_owner(s.incl, kPgMax, k, o);
+    if (!s.keys[o]) return;
+    plan[o * kPgPlanWords + 1] = p;
+    a.refs[p] = 1;
+  });
 }
 
 // ---------------------------------------------------------------------------
 // contents
 // ---------------------------------------------------------------------------
 // One piece of a page's head, all loads of a thread in flight before its first store.
-__device__ __forceinline__ void pg_copy_piece(const uint4* __restrict__ src, uint4* __restrict__ dst, int vecs) {
-  if (vecs >= kPgPieceVecs) {
-    uint4 v[kPgPieceVecs / kPgThreads];
+__device__ __forceinline__ void pg_copy_piece(const uint4* src, uint4* dst, int vecs) {
+  constexpr int kEach = kPgPieceVecs / kPgThreads;
+  uint4 v[kEach];
 #pragma unroll
-    for (int i = 0; i < kPgPieceVecs / kPgThreads; ++i) v[i] = __ldcs(src + threadIdx.x + i * kPgThreads);
+  for (int i = 0; i < kEach; ++i)
+    if (threadIdx.x + i * kPgThreads < vecs) v[i] = src[threadIdx.x + i * kPgThreads];
 #pragma unroll
-    for (int i = 0; i < kPgPieceVecs / kPgThreads; ++i) __stcs(dst + threadIdx.x + i * kPgThreads, v[i]);
-    return;
-  }
-  for (int i = threadIdx.x; i < vecs; i += kPgThreads) __stcs(dst + i, __ldcs(src + i));
+  for (int i = 0; i < kEach; ++i)
+    if (threadIdx.x + i * kPgThreads < vecs) dst[threadIdx.x + i * kPgThreads] = v[i];
 }
 
 __device__ __forceinline__ long long pg_plane(const PageCache& c, int plane) {
@@ -398,16 +407,18 @@ __global__ void __launch_bounds__(kPgMax, 1)
   __shared__ int s_holes;
   griddep_wait();
   griddep_launch_dependents();
-  int beg, end, free_pages;
-  pg_stretch(a.pages, beg, end);
-  const int mine = pg_count_free(a.refs, beg, end);
-  const int before = pg_scan(mine, sums, free_pages) - mine;  // free pages before the stretch
+  int free_pages;
+  const PgFree mine = pg_free_pages(a.refs, a.pages);
+  const int beg = mine.beg, end = mine.end;
+  const bool few = end - beg <= 64;
+  auto free_at = [&](int p) { return few ? (mine.bits >> (p - beg) & 1) != 0 : a.refs[p] == 0; };
+  const int before = pg_scan(mine.count, sums, free_pages) - mine.count;  // free pages before the stretch
   const int live = a.pages - free_pages;
   // holes: free pages among the first `live` places
   if (threadIdx.x == 0 && live == a.pages) s_holes = 0;
   if (beg <= live && live < end) {
     int h = before;
-    for (int p = beg; p < live; ++p) h += a.refs[p] == 0;
+    for (int p = beg; p < live; ++p) h += free_at(p);
     s_holes = h;
   }
   __syncthreads();
@@ -415,7 +426,7 @@ __global__ void __launch_bounds__(kPgMax, 1)
   if (threadIdx.x == 0) moves[0] = holes;
   int f = before;
   for (int p = beg; p < end; ++p) {
-    const bool is_free = a.refs[p] == 0;
+    const bool is_free = free_at(p);
     if (p < live) {
       if (is_free) moves[2 + 2 * f + 1] = p;  // the f-th hole
       place[p] = is_free ? -1 : p;
