@@ -151,25 +151,6 @@ __device__ __forceinline__ bool sp_elect() {
   return p != 0;
 }
 
-// 2^y of two values on the FMA pipe: n = round(y), 2^n from its bits, 2^(y - n)
-// by the polynomial of degree 4 that is best on [-1/2, 1/2] (its relative error,
-// found by exchange, is 2.7e-6).  Below -127 the result is 0; NaN stays NaN.
-__device__ __forceinline__ F2 sp_exp2_fma(F2 y) {
-  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: y + kRound has n in its low bits
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y.x) : "f"(-127.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y.y) : "f"(-127.f));
-  const F2 t = sp_add2(y, {kRound, kRound});
-  const F2 n = sp_add2(t, {-kRound, -kRound});
-  const F2 f = sp_fma2(n, {-1.f, -1.f}, y);
-  F2 p = {0.00957010220736265f, 0.00957010220736265f};
-  p = sp_fma2(p, f, {0.05591785907745361f, 0.05591785907745361f});
-  p = sp_fma2(p, f, {0.240247443318367f, 0.240247443318367f});
-  p = sp_fma2(p, f, {0.6931217908859253f, 0.6931217908859253f});
-  p = sp_fma2(p, f, {0.9999992847442627f, 0.9999992847442627f});
-  const F2 s = {__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
-                __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)};
-  return sp_fma2(p, s, {0.f, 0.f});
-}
 __device__ __forceinline__ float sp_max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -728,12 +709,9 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const F2 y = sp_fma2({s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]}, scale2, minus);
-            // three pairs of eight on the FMA pipe: the exponential unit alone
-            // would take as long as the products
-            const bool fma = (i & 7) == 1 || (i & 7) == 4 || (i & 7) == 6;
-            F2 e;
-            if (fma) e = sp_exp2_fma(y);
-            else e = {sp_exp2(y.x), sp_exp2(y.y)};
+            // (a polynomial on the FMA pipe for some of the pairs: 2 % faster for
+            // one of eight, 5 % slower for three, the warps then lack issue slots)
+            const F2 e = {sp_exp2(y.x), sp_exp2(y.y)};
             sum[i & 3] = sp_add2(sum[i & 3], e);
             pk[i] = pack_bf16x2(e.x, e.y);
           }
