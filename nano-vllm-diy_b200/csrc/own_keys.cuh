@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
     tma_prefetch_desc(&tmQ);
   }
   // A CTA that comes late (its SM had a job of the prefix) and finds the queue
-  // empty needs no plan.
-  {
+  // empty needs no plan.  (CTA 0 leaves the merge the first items: it always has one.)
+  if (blockIdx.x != 0) {
     __shared__ int s_late;
     if (tid == 0) {
       const int items = *reinterpret_cast<volatile int*>(&a.queue[2]) - 1;
@@ -133,10 +133,11 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
     for (int b = beg; b < end; ++b) {
       const int g = sp_group_of(a, b);
       const int p = g >= 0 ? sp_shared_pages(a, a.prefix_len[g], cnt[g], least[g]) * a.page : 0;
-      const int nq = a.cu_q[b + 1] - a.cu_q[b];
+      const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0;
       const int nk = a.cu_k[b + 1] - a.cu_k[b] - p;
       s.prefix[b] = p;
-      s.start[b] = nq >= 1 ? max(nk, 0) : 0;  // own keys, for now
+      // own keys, for now (a row outside q has no place to go: sp_group_of reports it)
+      s.start[b] = nq >= 1 && q0 >= 0 && q0 < a.num_q_rows ? max(nk, 0) : 0;
       keys += s.start[b];
       active += s.start[b] > 0;
     }
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
 constexpr int kMergeWarps = 4;
 
 template <int kFlight>
-__global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 10) shared_merge_kernel(const SharedArgs a) {
+__global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 9) shared_merge_kernel(const SharedArgs a) {
   griddep_wait();
   griddep_launch_dependents();
   const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -452,6 +453,11 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 10) share
   const int c0 = a.starts[b], own = a.starts[b + 1] - c0;
   const SpRec rc = a.rec[b];
   if (nq < 1 || (own == 1 && rc.keys == 0)) return;  // padding; written by its one item
+  if (q0 < 0 || q0 >= a.num_q_rows) return;            // reported by the prefix kernel
+  if (c0 < 0 || own < 0 || (long long)c0 + own > a.cap_items) {  // lengths past max_seqlen_k: no such parts
+    if (lane == 0) raise_error(a.err, ERR_BAD_INDEX);
+    return;
+  }
   const int pieces = rc.keys > 0 ? rc.split : 0;  // of the prefix: the first, then those of the next jobs
   const int job = rc.off + (h * rc.blocks + rc.rank / a.members) * rc.split;
   const size_t first = ((size_t)rc.start * a.Hkv + (size_t)h * rc.members + rc.rank) * a.G + (hq - h * a.G);

@@ -286,6 +286,37 @@ def test_missing_pages_count_for_nothing_and_are_flagged():
     assert b200.device_error(clear=True) == 4
 
 
+def test_lengths_past_max_seqlen_k_are_flagged():
+    """More own keys than max_seqlen_k allows for: the error word says so, nothing
+    is read or written out of place, and the next call is right."""
+    from src import b200
+    b = Batch(8, 8, [], alone=[1400], seed=2)
+    n = 300
+    b.table = b.table.expand(n, -1).contiguous()
+    b.q = torch.randn(n, 8, 128, generator=torch.Generator().manual_seed(3)).to(BF).to(DEV)
+    b.cu_q = i32(list(range(n + 1)))
+    b.cu_k = i32([1400 * i for i in range(n + 1)])
+    b.B, b.live, b.lens, b.group = n, n, [1400] * n, [-1] * n
+    out = torch.full((n + 1, 8, 128), 7.0, dtype=BF, device=DEV)
+    b.run(max_k=1, out=out[:n])
+    assert b200.device_error(clear=True) == 4
+    assert bool((out[n] == 7.0).all())
+    b.check(b.run(), range(0, n, 30))
+
+
+@pytest.mark.parametrize("group", [-1, 0])
+def test_rows_outside_q_are_flagged(group):
+    """A sequence whose query row lies behind q is left out, the others are answered."""
+    from src import b200
+    b = Batch(8, 2, [(512, 512, [3, 700, 5, 9])], alone=[300], seed=4)
+    b.group[-1] = group
+    out = torch.full((b.B, 8, 128), 7.0, dtype=BF, device=DEV)
+    b.run(q=b.q[:-1], out=out[:-1], group=i32(b.group))
+    assert b200.device_error(clear=True) == 4
+    b.check(out, range(b.live - 1))
+    assert bool((out[-1] == 7.0).all())
+
+
 @pytest.mark.parametrize("B,prefix,Hq,Hkv", [(256, 8192, 32, 8), (1024, 1024, 16, 2)])
 def test_large_batches(B, prefix, Hq, Hkv):
     g = torch.Generator().manual_seed(B)
