@@ -1578,12 +1578,12 @@ SharedLayout shared_layout(int num_sms, int seqs, int max_seqlen_k, int Hq, int 
 
 // The softmax warps raise their register count to what the launch has to give:
 // a build in which the kernel takes fewer registers must not start.
-int check_prefix_registers() {
+int check_shared_registers() {
   static int regs = 0;
   std::lock_guard<std::mutex> lock(g_host_mutex);
   if (regs == 0) {
     cudaFuncAttributes f{};
-    const cudaError_t e = cudaFuncGetAttributes(&f, shared_prefix_kernel);
+    const cudaError_t e = cudaFuncGetAttributes(&f, shared_attention_kernel);
     if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix: %s", cudaGetErrorString(e));
     regs = f.numRegs;
   }
@@ -1678,23 +1678,18 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   s.rest_ml = reinterpret_cast<float2*>(ws + l.rest_ml);
   s.rest_o = reinterpret_cast<float*>(ws + l.rest_o);
   s.err = ds->err;
-  // the shared part
+  // prefixes and own keys (one kernel, one box: tiles of 32 keys)
   if (int r = make_tmap_3d(&tmK, k_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kOwnTile)) return r;
   if (int r = make_tmap_3d(&tmV, v_cache, kOwnHD, Hkv, (uint64_t)num_slots, kOwnHD * 2, row, 64, 1, kOwnTile)) return r;
-  if (int r = check_prefix_registers()) return r;
-  if (int r = ensure_smem(ds, 32u, shared_prefix_kernel, kSpSmemBytes)) return r;
-  cudaError_t e = launch_ex(shared_prefix_kernel, dim3(ds->num_sms), dim3(kSpThreads), kSpSmemBytes, st, nullptr, 0,
-                            tmK, tmV, s);
-  if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
-  if (int r = check_launch("shared_prefix_kernel")) return r;
-  // every sequence's own keys
   if (int r = make_tmap_3d(&tmQ, q, kOwnHD, Hq, (uint64_t)num_q_rows, kOwnHD * 2, (uint64_t)q_stride * 2, 64,
                            (uint32_t)std::min(Hq, 8), 1))
     return r;
-  if (int r = ensure_smem(ds, 64u, own_keys_kernel, kOwnSmemBytes)) return r;
-  e = launch_overlapped(own_keys_kernel, ds->num_sms, kOwnThreads, kOwnSmemBytes, st, tmK, tmV, tmQ, s);
+  if (int r = check_shared_registers()) return r;
+  if (int r = ensure_smem(ds, 32u, shared_attention_kernel, kSharedSmemBytes)) return r;
+  cudaError_t e = launch_ex(shared_attention_kernel, dim3(ds->num_sms), dim3(kSpThreads), kSharedSmemBytes, st,
+                            nullptr, 0, tmK, tmV, tmQ, s);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
-  if (int r = check_launch("own_keys_kernel")) return r;
+  if (int r = check_launch("shared_attention_kernel")) return r;
   // the parts of each row
   const int rows = B * Hq;
   e = launch_overlapped(rows <= ds->num_sms * 24 ? shared_merge_kernel<8> : shared_merge_kernel<4>,

@@ -49,12 +49,16 @@ struct OwnPlan {
   long long keys[kOwnThreads / 32];
   int sums[kOwnThreads / 32];
   int item;                   // keys of an item
+  int late;
   int start[kSpMaxSeqs + 1];  // first item (of one kv head) of each sequence
   int prefix[kSpMaxSeqs];     // keys of its shared prefix
 };
-constexpr int kOwnSmemBytes = 1024 + kOwnWarps * kOwnWarpBytes + (int)sizeof(OwnPlan);
-static_assert(kOwnSmemBytes <= 227 * 1024, "shared memory of one CTA");
-static_assert(2 * kSpMaxGroups * 4 + 8 <= kOwnWarps * kOwnWarpBytes, "the counts fit the rings");
+static_assert(kOwnThreads == kSpThreads, "one CTA does both");
+constexpr int kOwnPlanAt = kOwnWarps * kOwnWarpBytes;
+static_assert(kOwnPlanAt >= kSpPlanAt + (int)sizeof(SpPlan), "behind all that the jobs use");
+static_assert(kOwnPlanAt + (int)sizeof(OwnPlan) <= kSpBar, "the jobs' barriers stay");
+constexpr int kSharedSmemBytes = 1024 + kSpBar + 256;
+static_assert(kSharedSmemBytes <= 227 * 1024, "shared memory of one CTA");
 
 // Tiled load of keys that no one else will read: they leave L2 first, before
 // the shared prefixes, the partials and the kernels' own instructions.
@@ -86,53 +90,36 @@ __device__ __forceinline__ void own_leave(const SharedArgs& a, int n) {
   }
 }
 
-__global__ void __launch_bounds__(kOwnThreads, 1)
-    own_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                    const __grid_constant__ CUtensorMap tmQ, const SharedArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  OwnPlan& s = *reinterpret_cast<OwnPlan*>(smem + kOwnWarps * kOwnWarpBytes);
+// The own keys, as many items as this CTA gets from the queue.  All threads call
+// it, after the jobs of the prefixes; `sp` is the plan of those, whose memory the
+// rings take.
+__device__ __forceinline__ void own_run(const SharedArgs& a, uint8_t* smem, const SpPlan& sp, const CUtensorMap& tmK,
+                                        const CUtensorMap& tmV, const CUtensorMap& tmQ) {
+  OwnPlan& s = *reinterpret_cast<OwnPlan*>(smem + kOwnPlanAt);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < kOwnWarps * kOwnStages) {
-    mbar_init(&s.full[0][tid], 1);
-    mbar_init(&s.empty[0][tid], 1);
-    fence_mbar_init();
-  }
-  if (tid == 0) {
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
-    tma_prefetch_desc(&tmQ);
-  }
-  // A CTA that comes late (its SM had a job of the prefix) and finds the queue
-  // empty needs no plan.  (CTA 0 leaves the merge the first items: it always has one.)
-  if (blockIdx.x != 0) {
-    __shared__ int s_late;
+  // the CTA whose number no job has, unless every SM has one, writes what the merge reads
+  const bool writer = blockIdx.x == gridDim.x - 1;
+  // A CTA that comes late (it had a job) and finds the queue empty needs no plan.
+  if (!writer) {
     if (tid == 0) {
       const int items = *reinterpret_cast<volatile int*>(&a.queue[2]) - 1;
-      s_late = items >= 0 && *reinterpret_cast<volatile int*>(&a.queue[0]) >= items;
+      s.late = items >= 0 && *reinterpret_cast<volatile int*>(&a.queue[0]) >= items;
     }
     __syncthreads();
-    if (s_late) {
+    if (s.late) {
       if (tid == 0) own_leave(a, kOwnWarps);
-      griddep_launch_dependents();
-      griddep_wait();
       return;
     }
   }
-  // ---- plan (every CTA the same): shared keys, then the prefix sum of items.
-  // The inputs are older than the prefix kernel, which waited for them.
+  // ---- plan (every CTA the same): shared keys, then the prefix sum of items
   {
-    int* cnt = reinterpret_cast<int*>(smem);  // in the rings, before their first load
-    int* least = cnt + kSpMaxGroups;
-    unsigned long long* all = reinterpret_cast<unsigned long long*>(least + kSpMaxGroups);
-    sp_count_groups(a, cnt, least, all, nullptr, kOwnThreads);
     const int per = (a.B + kOwnThreads - 1) / kOwnThreads;
     const int beg = min(a.B, tid * per), end = min(a.B, beg + per);
     long long keys = 0;
     int active = 0;
     for (int b = beg; b < end; ++b) {
       const int g = sp_group_of(a, b);
-      const int p = g >= 0 ? sp_shared_pages(a, a.prefix_len[g], cnt[g], least[g]) * a.page : 0;
+      const int p = g >= 0 ? sp.tiles[g] * kSpTile : 0;
       const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0;
       const int nk = a.cu_k[b + 1] - a.cu_k[b] - p;
       s.prefix[b] = p;
@@ -188,11 +175,10 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
     __syncthreads();
   }
   const int total = s.start[a.B], len = s.item;
-  if (blockIdx.x == 0)
+  if (writer)
     for (int b = tid; b <= a.B; b += kOwnThreads) a.starts[b] = s.start[b];
   if ((long long)total > a.cap_items) {  // lengths past max_seqlen_k
-    if (blockIdx.x == 0 && tid == 0) raise_error(a.err, ERR_BAD_INDEX);
-    griddep_wait();
+    if (writer && tid == 0) raise_error(a.err, ERR_BAD_INDEX);
     return;
   }
   const int w = warp % kOwnWarps;
@@ -429,8 +415,41 @@ __global__ void __launch_bounds__(kOwnThreads, 1)
       }
     }
   }
+}
+
+// Jobs of the shared prefixes, then own keys: a CTA without a job starts on the
+// own keys at once.  (Two kernels that overlapped took 3 us more: the second one's
+// CTAs began where the first one's ended, and made the plan once more.)
+__global__ void __launch_bounds__(kSpThreads, 1)
+    shared_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                            const __grid_constant__ CUtensorMap tmQ, const SharedArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const SpSmem sm(smem);
+  const int tid = threadIdx.x;
+  if (tid == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmQ);
+    sm.init();
+  }
+  if (tid >= 32 && tid < 32 + kOwnWarps * kOwnStages) {
+    OwnPlan& s = *reinterpret_cast<OwnPlan*>(smem + kOwnPlanAt);
+    mbar_init(&s.full[0][tid - 32], 1);
+    mbar_init(&s.empty[0][tid - 32], 1);
+  }
+  fence_mbar_init();
+  griddep_wait();
+  SpDraft& draft = *reinterpret_cast<SpDraft*>(smem + kSpRing);
+  sp_build_plan(a, sm.plan(), draft);
+  const int jobs = sm.plan().off[a.groups];
+  if (blockIdx.x == gridDim.x - 1) sp_write_records(a, sm.plan(), draft);
+  // the ring, with the draft in it, is the TMA's from here on
+  fence_proxy_async_smem();
+  __syncthreads();
+  if ((int)blockIdx.x < jobs) sp_run_jobs(a, sm, jobs, tmK, tmV);
+  own_run(a, smem, sm.plan(), tmK, tmV, tmQ);
   griddep_launch_dependents();
-  griddep_wait();  // so that the end of this grid is the prefix kernel's too
 }
 
 // ---------------------------------------------------------------------------

@@ -52,8 +52,8 @@ static_assert(kSpRegsIssue + 2 * kSpRegsSoftmax == 3 * kSpRegsLaunch, "the share
 constexpr float kSpLazy = 8.f;
 constexpr int kSpQ = 0;                            // [2 tiles][2 dim halves][128 rows][128 B]
 constexpr int kSpRing = 65536;
-constexpr int kSpBar = kSpRing + kSpSlots * 32768;
-constexpr int kSpPlanAt = kSpBar + 256;
+constexpr int kSpPlanAt = kSpRing + kSpSlots * 32768;
+constexpr int kSpBar = 226 * 1024 - 256;           // behind everything else: no other use of the memory
 
 // The groups of a call, in shared memory.
 struct SpPlan {
@@ -72,8 +72,6 @@ struct SpDraft {
   short rank[kSpMaxSeqs];
   short seen[kSpMaxGroups];         // members numbered so far
 };
-constexpr int kSpSmemBytes = 1024 + kSpPlanAt + (int)sizeof(SpPlan);
-static_assert(kSpSmemBytes <= 227 * 1024, "shared memory of one CTA");
 static_assert(sizeof(SpDraft) <= kSpSlots * 32768, "the draft fits the ring");
 
 // What the merge needs of a sequence; keys = 0: no shared part.
@@ -423,66 +421,68 @@ __device__ __forceinline__ long long sp_tile_row(const SharedArgs& a, int leader
   return blk >= 0 && row + kSpTile <= a.num_slots ? row : -1;
 }
 
-__global__ void __launch_bounds__(kSpThreads, 1)
-    shared_prefix_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                         const SharedArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSpBar);
-  uint64_t* full = bars;                   // [kSpSlots]
-  uint64_t* empty = bars + kSpSlots;       // [kSpSlots]
-  uint64_t* q_full = bars + 2 * kSpSlots;  // [2] a job's query rows are in shared memory, O may be overwritten
-  uint64_t* s_full = q_full + 2;           // [2]
-  uint64_t* p_full = q_full + 4;           // [2]
-  uint64_t* o_done = q_full + 6;           // [2]
-  uint64_t* p_half = q_full + 8;           // [2] the first 64 keys of P are there
-  uint64_t* drain = q_full + 10;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 11);
-  volatile int* bad = reinterpret_cast<int*>(q_full + 12);  // some page is missing: the softmax looks which
-  SpPlan& plan = *reinterpret_cast<SpPlan*>(smem + kSpPlanAt);
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-
-  if (threadIdx.x == 0) {
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
+// Shared memory of the jobs, aligned to 1024 bytes.
+struct SpSmem {
+  uint8_t* smem;
+  uint64_t* bars;
+  __device__ __forceinline__ explicit SpSmem(uint8_t* p) : smem(p), bars(reinterpret_cast<uint64_t*>(p + kSpBar)) {}
+  __device__ __forceinline__ uint64_t* full() const { return bars; }                   // [kSpSlots]
+  __device__ __forceinline__ uint64_t* empty() const { return bars + kSpSlots; }       // [kSpSlots]
+  // [2] a job's query rows are in shared memory, O may be overwritten
+  __device__ __forceinline__ uint64_t* q_full() const { return bars + 2 * kSpSlots; }
+  __device__ __forceinline__ uint64_t* s_full() const { return q_full() + 2; }         // [2]
+  __device__ __forceinline__ uint64_t* p_full() const { return q_full() + 4; }         // [2]
+  __device__ __forceinline__ uint64_t* o_done() const { return q_full() + 6; }         // [2]
+  __device__ __forceinline__ uint64_t* p_half() const { return q_full() + 8; }         // [2] the first 64 keys of P are there
+  __device__ __forceinline__ uint64_t* drain() const { return q_full() + 10; }
+  __device__ __forceinline__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(q_full() + 11); }
+  // some page is missing: the softmax looks which
+  __device__ __forceinline__ volatile int* bad() const { return reinterpret_cast<int*>(q_full() + 12); }
+  __device__ __forceinline__ SpPlan& plan() const { return *reinterpret_cast<SpPlan*>(smem + kSpPlanAt); }
+  // One thread; the barrier that ends the plan shows them to the others.
+  __device__ __forceinline__ void init() const {
     for (int i = 0; i < 2 * kSpSlots; ++i) mbar_init(&bars[i], 1);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&q_full[t], 4);  // a warp's lane 0 arrives for its rows
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
-      mbar_init(&p_half[t], 4);
-      mbar_init(&o_done[t], 1);
+      mbar_init(&q_full()[t], 4);  // a warp's lane 0 arrives for its rows
+      mbar_init(&s_full()[t], 1);
+      mbar_init(&p_full()[t], 4);
+      mbar_init(&p_half()[t], 4);
+      mbar_init(&o_done()[t], 1);
     }
-    mbar_init(drain, 1);
-    *bad = 0;
-    fence_mbar_init();
+    mbar_init(drain(), 1);
+    *bad() = 0;
   }
-  griddep_wait();
-  griddep_launch_dependents();
-  SpDraft& draft = *reinterpret_cast<SpDraft*>(smem + kSpRing);
-  sp_build_plan(a, plan, draft);
-  const int jobs = plan.off[a.groups];
-  if (blockIdx.x == 0) {
-    // what the merge needs
-    for (int b = threadIdx.x; b < a.B; b += kSpThreads) {
-      SpRec r{};
-      const int g = draft.group[b];
-      if (g >= 0 && plan.tiles[g] > 0) {
-        r.keys = plan.tiles[g] * kSpTile;
-        r.split = plan.split[g];
-        r.off = plan.off[g];
-        r.start = plan.start[g];
-        r.members = plan.start[g + 1] - plan.start[g];
-        r.blocks = sp_div(r.members + a.members - 1, a.members);
-        r.rank = draft.rank[b];
-      }
-      a.rec[b] = r;
+};
+
+// What the merge needs of the sequences; all threads of a CTA call it after the plan.
+__device__ __forceinline__ void sp_write_records(const SharedArgs& a, const SpPlan& plan, const SpDraft& draft) {
+  for (int b = threadIdx.x; b < a.B; b += kSpThreads) {
+    SpRec r{};
+    const int g = draft.group[b];
+    if (g >= 0 && plan.tiles[g] > 0) {
+      r.keys = plan.tiles[g] * kSpTile;
+      r.split = plan.split[g];
+      r.off = plan.off[g];
+      r.start = plan.start[g];
+      r.members = plan.start[g + 1] - plan.start[g];
+      r.blocks = sp_div(r.members + a.members - 1, a.members);
+      r.rank = draft.rank[b];
     }
+    a.rec[b] = r;
   }
-  // the ring, with the draft in it, is the TMA's from here on
-  fence_proxy_async_smem();
-  __syncthreads();
-  if ((int)blockIdx.x >= jobs) return;  // the whole CTA, before any TMEM
+}
+
+// This CTA's jobs: number blockIdx.x, and every gridDim.x-th after it.  All
+// threads call it, with the registers of the launch, and have those again after it.
+__device__ __forceinline__ void sp_run_jobs(const SharedArgs& a, const SpSmem& sm, int jobs, const CUtensorMap& tmK,
+                                            const CUtensorMap& tmV) {
+  uint8_t* smem = sm.smem;
+  uint64_t *full = sm.full(), *empty = sm.empty(), *q_full = sm.q_full(), *s_full = sm.s_full(),
+           *p_full = sm.p_full(), *o_done = sm.o_done(), *p_half = sm.p_half(), *drain = sm.drain();
+  uint32_t* tmem_slot = sm.tmem_slot();
+  volatile int* bad = sm.bad();
+  SpPlan& plan = sm.plan();
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t base = smem_u32(smem);
 
   if (warp < 4) {
@@ -524,6 +524,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       for (int i = it > kSpSlots ? it - kSpSlots : 0; i < it; ++i)
         mbar_wait(&full[i % kSpSlots], (uint32_t)(i / kSpSlots) & 1u, a.err);
     }
+    __syncwarp();
     // ---- MMA issuer: the whole warp walks the loop, so that descriptors live in
     // uniform registers, and one elected lane issues
     if (warp == 1) {
@@ -767,9 +768,14 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(*tmem_slot, 512);
+  if (warp < 4) {
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(*tmem_slot, 512);
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSpRegsLaunch));
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSpRegsLaunch));
   }
 }
 
