@@ -8,14 +8,14 @@
 // so this kernel computes the partials of all members over the group's prefix
 // at once -- a dense product of (members x heads) query rows with the prefix
 // keys on the tensor cores, each K / V byte read once for up to 256 rows --,
-// decode_attn_kernel<true> then streams every sequence's own keys and merges.
+// the same CTAs then stream every sequence's own keys (own_keys.cuh).
 //
 // Work: a row block is up to 256 rows of one group and kv head (256 / G members x
 // the G = Hq / Hkv heads) and its prefix in tiles of 128 keys.  A job is a row
 // block's whole prefix, or one of the equal pieces it is cut into so that no
 // SM idles: a CTA (one on each SM) does one job as long as there are no more
 // jobs than SMs.  How long the pieces are is weighed against the own keys,
-// whose kernel runs on the SMs that get no job (sp_choose_piece).  The piece
+// on which the SMs without a job start at once (sp_choose_piece).  The piece
 // that starts a row block leaves its partial in the rows of the sequences, the
 // others in a slot of their job: no place is written twice, and the merge finds
 // them by the same arithmetic, in a fixed order.
@@ -257,29 +257,36 @@ __device__ __forceinline__ void sp_count_groups(const SharedArgs& a, int* cnt, i
   __syncthreads();
 }
 
-// Pages of a group's prefix that count: whole ones that every member sees.  The
-// prefix is shared where that pays: reading a tile (64 KB) once instead of once
-// a member saves 10.7 ns of HBM's time at 6.1 TB/s, and a job costs an SM about
-// 11 us and 2.15 us a tile.  So pairs never share, four members from 5 tiles on,
-// eight from 2 (measured: 64 pairs behind 512 keys 101 us shared and 74 not, 16
-// groups of 4 behind 512 38 and 33; 64 groups of 4 behind 2k 146 and 223).
-__device__ __forceinline__ int sp_shared_pages(const SharedArgs& a, int given, int members, int least) {
-  if (members < 2) return 0;
-  const int pages = min(max(min(given, least), 0) / a.page, a.bt_width);
-  // (in whole numbers: both kernels have to come to the same answer)
-  const long long tiles = (long long)pages * (a.page / kSpTile);
-  const long long saved = (members - 1) * tiles * 159;  // 0.01 us of one of 148 SMs
-  const long long cost = sp_div(members + a.members - 1, a.members) * (1100 + 215 * tiles);
-  return saved > cost || a.always ? pages : 0;
+// A job takes about kSpCostJob + kSpCostTile a tile (us), own keys begin after kSpCostOwn.
+constexpr float kSpCostJob = 14.f, kSpCostTile = 2.2f, kSpCostOwn = 10.f;
+
+// Tiles of a group's prefix: of whole pages that every member sees.
+__device__ __forceinline__ int sp_prefix_tiles(const SharedArgs& a, int given, int members, int least) {
+  return members < 2 ? 0 : min(max(min(given, least), 0) / a.page, a.bt_width) * (a.page / kSpTile);
+}
+
+// A prefix is shared where that pays, by times in us:
+// - Reading a tile (64 KB) once and not once a member saves 1.59 of an SM for
+//   each member but one; a row block costs 15 beside the reads and 0.6 a tile.
+// - A job, cut into as many pieces as the SMs have room for, has to be over before
+//   the batch without sharing would be (`alone` to read all keys, of which a
+//   part is shared elsewhere: 0.6 of it; 2 more than a job's start).
+// Measured, shared / not: 64 pairs behind 0.1 to 0.5k keys 79 / 57, 0.5 to 2k
+// 122 / 125, 1 to 4k 183 / 210; 128 pairs behind 1 to 4k 344 / 431; 16 pairs behind 1
+// to 4k 71 / 54 (the second rule: 128 jobs, uncut); 64 groups of 4 behind 0.5 to 2k
+// 140 / 211.
+__device__ __forceinline__ bool sp_pays(const SharedArgs& a, int tiles, int members, int blocks, int pieces,
+                                        float alone) {
+  const float saved = 1.59f * (float)(members - 1) * (float)tiles;
+  const float cost = (float)blocks * (15.f + 0.6f * (float)tiles);
+  const float job = kSpCostJob + kSpCostTile * (float)sp_div(tiles + pieces - 1, pieces);
+  return saved > cost && job < 0.6f * alone + kSpCostJob + 2.f;
 }
 
 // Tiles of a piece, chosen by one warp: each lane weighs one number of pieces of
-// the longest prefix by a model of both kernels, fitted to measurements (us, on
-// 148 SMs).  A CTA of this kernel takes about kSpCostJob + kSpCostTile a tile;
-// an SM streams own keys at 60 GB/s, all of them together at 6.1 TB/s, and the
-// own-keys kernel takes the SMs without a job at once and the others when
-// their jobs end.
-constexpr float kSpCostJob = 14.f, kSpCostTile = 2.2f, kSpCostOwn = 10.f;
+// the longest prefix by a model of the call, fitted to measurements (us, on 148
+// SMs): an SM streams own keys at 60 GB/s, all of them together at 6.1 TB/s, the
+// SMs without a job from the start and the others when their jobs end.
 __device__ __forceinline__ int sp_choose_piece(const SharedArgs& a, const SpPlan& s, const SpDraft& d, int longest,
                                               long long own_keys) {
   const int lane = threadIdx.x & 31, sms = gridDim.x;
@@ -332,10 +339,19 @@ __device__ __forceinline__ void sp_build_plan(const SharedArgs& a, SpPlan& s, Sp
   }
   if (tid < 32) {
     // prefixes, then the length of a piece, then first members and jobs
-    int longest = 0;
+    int longest = 0, blocks = 0;
     long long shared_keys = 0;
     for (int g = lane; g < a.groups; g += 32) {
-      const int tiles = sp_shared_pages(a, s.tiles[g], d.cnt[g], d.least[g]) * (a.page / kSpTile);
+      s.tiles[g] = sp_prefix_tiles(a, s.tiles[g], d.cnt[g], d.least[g]);
+      if (s.tiles[g] > 0) blocks += sp_div(d.cnt[g] + a.members - 1, a.members);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) blocks += __shfl_xor_sync(0xffffffffu, blocks, o);
+    const int room = blocks > 0 ? max(1, sp_div(gridDim.x, blocks * a.Hkv)) : 1;
+    const float alone = (float)d.keys * (float)(a.Hkv * 512) / 6.1e6f;
+    for (int g = lane; g < a.groups; g += 32) {
+      int tiles = s.tiles[g];
+      if (!a.always && !sp_pays(a, tiles, d.cnt[g], sp_div(d.cnt[g] + a.members - 1, a.members), room, alone)) tiles = 0;
       s.tiles[g] = tiles;
       longest = max(longest, tiles);
       shared_keys += (long long)d.cnt[g] * tiles * kSpTile;
