@@ -52,8 +52,9 @@ unsigned long long b200_launch_count(void);
 /* Reads the device error word of the current device; clears it when `clear`
  * is non-zero.  Synchronous.  After a timeout bit (a bounded wait gave up),
  * zero the first b200_attention_workspace_bytes(0, 0, 1) bytes of the
- * attention workspace and the first 4096 bytes of the GEMM workspace before
- * the next call: the kernel that gave up can leave counters behind. */
+ * attention workspace, the first 4096 bytes of the GEMM workspace and the
+ * first 256 of the shared-prefix workspace before the next call: the kernel
+ * that gave up can leave counters behind. */
 int b200_device_error(unsigned* out, int clear);
 
 /* ------------------------------------------------------------------------
@@ -306,6 +307,10 @@ int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, i
  *    keys gives zeros; rows with q length <= 0 (padding) are left alone.
  *  - B <= 1024, num_groups <= 512, Hq / Hkv <= 8, page a multiple of 256,
  *    softmax_scale > 0.
+ *  - Sequences longer than max_seqlen_k may not fit the workspace's places for
+ *    parts of a row; then B200_DEVERR_BAD_INDEX is set and the output is not
+ *    to be used.  It is also set for a query row outside q (left out) and for
+ *    missing pages (their keys count for nothing).
  *  - workspace: b200_shared_prefix_workspace_bytes(B, max_seqlen_k, Hq, Hkv) bytes,
  *    256-byte aligned, its first 256 bytes zero before the first call (they
  *    are zero again after every call).  Calls that share a

@@ -13,9 +13,14 @@
 // tiles (TMA, 128-byte swizzle, one mbarrier each way) full, so that the queue's
 // and the tables' latency never stops the arithmetic; the consumer's chain of
 // products and shuffles is what a tile costs an SM, and six of them in flight
-// with two tiles each beat four with three.  The launch may overlap the prefix
-// kernel: it reads nothing that kernel writes, and takes the SMs it leaves free.
-// A row with several parts leaves them as fp32 partials (m, l, o).
+// with two tiles each beat four with three.  A row with several parts leaves them
+// as fp32 partials (m, l, o).
+//
+// Measured (32 query and 8 kv heads): 256 sequences behind one prefix of 8k keys,
+// 526 MB of own keys beside 64 jobs of 32 tiles, 99 us and 6 for the merge (the
+// bytes alone: 87); 256 sequences in 9 groups and without one, 665 MB, 126 us and
+// 8 (119); 32 sequences behind 2k keys, 48 MB, 18.5 and 6 (8.9: the plan takes 4
+// us, an item's first tile 3, the merge waits for the launch and two trips to L2).
 #pragma once
 #include "common.cuh"
 #include "shared_prefix.cuh"
@@ -418,8 +423,10 @@ __device__ __forceinline__ void own_run(const SharedArgs& a, uint8_t* smem, cons
 }
 
 // Jobs of the shared prefixes, then own keys: a CTA without a job starts on the
-// own keys at once.  (Two kernels that overlapped took 3 us more: the second one's
-// CTAs began where the first one's ended, and made the plan once more.)
+// own keys at once.  (Two kernels that overlapped took 1 to 3 us more: the second
+// one's CTAs began where the first one's ended, and made the plan once more.  The
+// merge behind a barrier of all CTAs in this kernel, instead of a launch of its
+// own, took 1 to 3 us more, too: 12 resident warps an SM, not 36.)
 __global__ void __launch_bounds__(kSpThreads, 1)
     shared_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                             const __grid_constant__ CUtensorMap tmQ, const SharedArgs a) {
@@ -472,7 +479,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 9) shared
   const int c0 = a.starts[b], own = a.starts[b + 1] - c0;
   const SpRec rc = a.rec[b];
   if (nq < 1 || (own == 1 && rc.keys == 0)) return;  // padding; written by its one item
-  if (q0 < 0 || q0 >= a.num_q_rows) return;            // reported by the prefix kernel
+  if (q0 < 0 || q0 >= a.num_q_rows) return;            // reported with the plan
   if (c0 < 0 || own < 0 || (long long)c0 + own > a.cap_items) {  // lengths past max_seqlen_k: no such parts
     if (lane == 0) raise_error(a.err, ERR_BAD_INDEX);
     return;

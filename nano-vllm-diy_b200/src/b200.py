@@ -238,7 +238,7 @@ def launch_count() -> int:
 _TIMEOUT_BITS = 0x1 | 0x2
 # the GEMM workspace starts with 4 KiB of split-K flags and counters
 _GEMM_FLAG_BYTES = 4096
-# the shared-prefix workspace starts with the queue of its own-keys kernel
+# the shared-prefix workspace starts with the queue of the own keys
 _QUEUE_BYTES = 256
 
 

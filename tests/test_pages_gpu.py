@@ -311,3 +311,41 @@ def test_pool_step_matches_host_metadata():
         for r, c in zip(rows, counts):
             lens[r] += c
         assert pool.seq_lens.tolist() == lens
+
+
+def test_many_pages():
+    """A pool of more than 65,536 pages, whose free pages are searched in the
+    counts themselves, and rows of thousands of pages."""
+    pool, model = make((1, 70001, 16, 1, 8), 40, 2000, seed=9)
+    lens = [16 * 1900 + 5 * i for i in range(36)]
+    for x in (pool, model):
+        done = x.take(list(range(36)), lens)
+        x.free(list(range(1, 36, 2)))
+    assert torch.as_tensor(done).tolist() == [1] * 36
+    same(pool, model)
+    assert pool.fork([0, 2, 34], [1, 3, 36]).tolist() == model.fork([0, 2, 34], [1, 3, 36])
+    calls = [[5, 7, 8, 9, 37, 38], [16 * 2000, 1, 16 * 1999, 16 * 1500, 3, 16 * 2000]]
+    assert pool.take(*calls).tolist() == model.take(*calls)
+    same(pool, model)
+    assert pool.compact().tolist() == model.compact()
+    same(pool, model)
+    pool.free(list(range(40)))
+    model.free(list(range(40)))
+    same(pool, model)
+    assert sum(model.refs) == 0
+
+
+def test_launches_that_may_overlap(monkeypatch):
+    """The same results where every launch may begin before the one in front of
+    it has ended."""
+    monkeypatch.setenv("B200_PDL", "1")
+    pool, model = make((2, 2, 64, 16, 2, 8), 12, 6, seed=10)
+    for _ in range(3):
+        for x in (pool, model):
+            x.take([0, 1, 2], [90, 33, 16])
+            x.fork([0, 1, 2, 0], [3, 4, 5, 6])
+            x.free([1, 3])
+            x.compact()
+            x.take([1, 3], [16, 7])
+            x.free([0, 1, 2, 3, 4, 5, 6])
+    same(pool, model)

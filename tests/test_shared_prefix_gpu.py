@@ -338,3 +338,41 @@ def test_on_another_stream():
         out = b.run()
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(out, want)
+
+
+def test_as_many_groups_as_there_can_be():
+    b = Batch(8, 1, [(256, 256, [3, 1 + i % 60]) for i in range(512)], seed=12)
+    b.check(b.run(), range(0, b.live, 11))
+
+
+def test_two_captured_graphs_with_one_workspace():
+    """Graphs of different batches replayed in turn: every call leaves the
+    workspace as the next one needs it."""
+    pair = [Batch(16, 2, [(1024, 1024, [40, 700, 3] * 6)], alone=[1500, 2], seed=13),
+            Batch(8, 8, [(512, 512, [90] * 5), (256, 256, [600, 1])], seed=14)]
+    outs = [torch.zeros_like(b.q) for b in pair]
+    index = [(i32(b.group), i32(b.prefix)) for b in pair]
+    for b, out, (g, p) in zip(pair, outs, index):
+        b.run(group=g, prefix=p, out=out)
+    want = [o.clone() for o in outs]
+    graphs = []
+    for b, out, (g, p) in zip(pair, outs, index):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            b.run(group=g, prefix=p, out=out)
+    for turn in (0, 1, 1, 0, 0, 1):
+        outs[turn].zero_()
+        graphs[turn].replay()
+        assert torch.equal(outs[turn], want[turn])
+    for b, out in zip(pair, outs):
+        b.check(out)
+
+
+def test_launches_that_may_overlap(monkeypatch):
+    monkeypatch.setenv("B200_PDL", "1")
+    b = Batch(8, 2, [(512, 512, [100, 200, 3, 900])], alone=[50], seed=15)
+    first = b.run()
+    for _ in range(4):
+        b.q.mul_(1.0)
+        assert torch.equal(b.run(), first)
+    b.check(first)

@@ -70,3 +70,23 @@ def test_custom_ops_run_the_same_kernels():
     assert torch.equal(torch.ops.b200.linear(x, w), b200.linear(x, w))
     logits = torch.randn(5, 1000, generator=g).to(BF).cuda()
     assert torch.equal(torch.ops.b200.argmax(logits), b200.argmax(logits))
+
+
+def test_fake_shapes_of_shared_prefixes_and_pages():
+    from src import torch_ops  # noqa: F401  (registers the ops)
+    ops = torch.ops.b200
+    with FakeTensorMode():
+        i32 = lambda *n: torch.empty(*n, dtype=torch.int32, device="cuda")  # noqa: E731
+        q = torch.empty(7, 32, 128, dtype=BF, device="cuda")
+        kv = torch.empty(2, 3, 9, 256, 8, 128, dtype=BF, device="cuda")
+        out = ops.shared_prefix_attention(q, kv[0, 0], kv[1, 0], i32(8), i32(8), 1024, 128 ** -0.5, i32(7, 4), i32(7),
+                                          i32(2))
+        assert out.shape == q.shape and out.dtype == BF
+        table, lens, refs = i32(7, 4), i32(7), i32(9)
+        assert ops.copy_pages(kv, i32(3), i32(3)) is None
+        assert ops.copy_pages(kv, i32(3), i32(3), i32(3)) is None
+        done = ops.take_pages(table, lens, refs, i32(3), i32(3), 256)
+        assert done.shape == (3,) and done.dtype == torch.int32
+        assert ops.free_pages(table, lens, refs, i32(2)) is None
+        assert ops.fork_pages(kv, table, lens, refs, i32(2), i32(2)).shape == (2,)
+        assert ops.compact_pages(kv, table, refs).shape == (9,)
