@@ -13,7 +13,8 @@ cache without the host reading anything back:
     positions, ctx, done = pool.step([0, 1, 2, 3], [1] * 4)  # one decode token each
     pool.free([2]); pool.compact()
 
-Rows are given as lists or as int32 device tensors; -1 entries are skipped.
+Rows are given as lists or as int32 device tensors; -1 entries are skipped
+(but not in a step).
 `done` is an int32 device tensor, 1 where the row got what it asked for (0
 when pages ran out, see src/b200.py).
 """
@@ -65,7 +66,14 @@ class PagePool:
     def step(self, rows, counts: list[int]) -> tuple[torch.Tensor, Context, torch.Tensor]:
         """Pages for counts[i] more tokens of each row and the step's metadata:
         (positions int64 [T], Context, done).  The Context is that of the rows
-        in the order given, as src/engine/metadata.py builds it."""
+        in the order given, as src/engine/metadata.py builds it.  Every row is
+        one of the pool's, named once: a step skips none (a row with done = 0 has
+        no page for its tokens: their slots are refused and flagged)."""
+        if not torch.is_tensor(rows) and (len(set(rows)) != len(rows) or
+                                          not all(0 <= r < self.seq_lens.shape[0] for r in rows)):
+            raise ValueError(f"step: rows {rows} of a pool of {self.seq_lens.shape[0]}, each once")
+        if len(counts) != len(rows) or not counts or min(counts) < 1:
+            raise ValueError(f"step: {len(counts)} token counts (of at least 1) for {len(rows)} rows")
         rows = self._vec(rows)
         at = rows.long()
         count = self._vec(counts)
@@ -73,7 +81,9 @@ class PagePool:
         done = self.take(rows, start + count)
         table = self.block_tables[at]
         end = start + count
-        info = torch.stack([start, count, (end + self.page - 1) // self.page])
+        # (a refused row may ask for more pages than a table has places)
+        held = torch.clamp((end + self.page - 1) // self.page, max=self.width)
+        info = torch.stack([start, count, held])
         total = sum(counts)
         positions, slots, cu_q, cu_k, lens = b200.step_metadata(info, table, self.page, total, total)
         most = max(counts)

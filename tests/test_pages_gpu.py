@@ -349,3 +349,21 @@ def test_launches_that_may_overlap(monkeypatch):
             x.take([1, 3], [16, 7])
             x.free([0, 1, 2, 3, 4, 5, 6])
     same(pool, model)
+
+
+def test_pool_step_past_the_longest_row_is_refused():
+    """A row that would outgrow its table keeps its pages and its length; its
+    tokens without a page have no slot, and the other rows get theirs."""
+    from src import b200
+    from src.engine.pages import PagePool
+    kv = torch.zeros(2, 1, 9, 16, 1, 8, dtype=torch.bfloat16, device=DEV)
+    pool = PagePool(kv, 3, 64)
+    pool.step([2, 0], [60, 17])
+    table = pool.block_tables.tolist()
+    positions, ctx, done = pool.step([0, 2], [2, 6])
+    assert done.tolist() == [1, 0] and b200.device_error(clear=True) == 4
+    assert pool.block_tables.tolist() == table and pool.seq_lens.tolist() == [19, 0, 60]
+    last = table[2][3] * 16
+    assert ctx.slot_mapping.tolist() == [table[0][1] * 16 + 1, table[0][1] * 16 + 2,
+                                         last + 12, last + 13, last + 14, last + 15, -1, -1]
+    assert positions.tolist() == [17, 18, 60, 61, 62, 63, 64, 65]

@@ -4,6 +4,7 @@ import random
 
 import numpy as np
 import pytest
+import torch
 
 
 def groups(tables, lens, block=256):
@@ -94,3 +95,13 @@ def test_a_thousand_nested_prefixes():
     group, prefix = groups(tables, [len(t) * 256 for t in tables])
     assert saved(group, prefix) >= 249 * 500 - 1000
     assert group.dtype == np.int32 and prefix.dtype == np.int32
+
+
+@pytest.mark.parametrize("rows,counts", [([0, -1], [1, 1]), ([0, 4], [1, 1]), ([2, 2], [1, 1]), ([0, 1, 2], [1]),
+                                         ([0, 1], [1, 0]), ([], [])])
+def test_pool_steps_refuse_rows_that_have_no_place(rows, counts):
+    from src.engine.pages import PagePool
+    pool = PagePool(torch.zeros(2, 1, 6, 16, 1, 8), 4, 64)
+    with pytest.raises(ValueError, match="step"):
+        pool.step(rows, counts)
+    assert pool.seq_lens.tolist() == [0] * 4
