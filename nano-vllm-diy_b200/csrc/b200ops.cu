@@ -1544,7 +1544,7 @@ size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 // Items (of the sequences' own keys) the workspace has room for: 512 keys each
 // and one more per sequence, or as many short ones as there are warps.
 long long shared_items(int num_sms, int seqs, int max_seqlen_k, int Hkv) {
-  return (long long)seqs * ((max_seqlen_k + kOwnItem - 1) / kOwnItem + 1) +
+  return (long long)seqs * (((long long)max_seqlen_k + kOwnItem - 1) / kOwnItem + 1) +
          ((long long)num_sms * kOwnWarps + Hkv - 1) / Hkv;
 }
 

@@ -671,21 +671,22 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise TypeError("block_table must be int32 [B, width] with contiguous rows")
     if table[0] != B:
         raise ValueError(f"block_table of {table[0]} rows for {B} sequences")
+    row = Hq * 128
     q_stride = q.stride()
-    if q_stride[1:] != (128, 1):
+    if q_stride[1:] != (128, 1) or q_stride[0] < row:  # (rows that overlap: one query for all sequences)
         q = q.contiguous()
         q_stride = q.stride()
     if out is None:
         out = torch.empty((T, Hq, 128), dtype=torch.bfloat16, device=q.device)
-    elif out.shape != q.shape or out.stride()[1:] != (128, 1):
-        raise ValueError(f"out must be {tuple(q.shape)} with contiguous heads")
+    elif out.shape != q.shape or out.stride()[1:] != (128, 1) or (T > 1 and out.stride(0) < row):
+        raise ValueError(f"out must be {tuple(q.shape)} with contiguous heads and rows apart")
     pages, page, Hkv, _ = cache
     max_k = int(max_seqlen_k)
     ws = _prefix_workspace(dev, B, max_k, Hq, Hkv)
-    _call("b200_shared_prefix_attention", dev, q.data_ptr(), q_stride[0], T, k_cache.data_ptr(), v_cache.data_ptr(),
+    _call("b200_shared_prefix_attention", dev, q.data_ptr(), q_stride[0] if T > 1 else row, T, k_cache.data_ptr(), v_cache.data_ptr(),
           pages * page, block_table.data_ptr(), stride[0], table[1], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
           B, max_k, Hq, Hkv, page, softmax_scale, prefix_group.data_ptr(), prefix_len.data_ptr(), groups,
-          out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel())
+          out.data_ptr(), out.stride(0) if T > 1 else row, ws.data_ptr(), ws.numel())
     return out
 
 

@@ -37,6 +37,11 @@ class ModelRunner:
         """shared_prefix: decode steps find the sequences whose block tables
         begin with the same blocks and attend over those once for all of them
         (b200.shared_prefix_attention)."""
+        if shared_prefix and (max_num_seqs > 1024 or block_size % 256 or
+                              config.num_attention_heads > 8 * config.num_key_value_heads):
+            raise ValueError("shared_prefix: at most 1024 sequences, blocks of a multiple of 256 tokens and 8 query "
+                             f"heads to a kv head (asked for {max_num_seqs}, {block_size}, "
+                             f"{config.num_attention_heads} to {config.num_key_value_heads})")
         self.config = config
         self.rank = rank
         self.world_size = world_size

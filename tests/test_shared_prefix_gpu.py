@@ -376,3 +376,49 @@ def test_launches_that_may_overlap(monkeypatch):
         b.q.mul_(1.0)
         assert torch.equal(b.run(), first)
     b.check(first)
+
+
+def test_one_query_for_all_sequences():
+    """q expanded over the batch (rows that lie on one another), and single rows
+    whose strides say nothing."""
+    from src import b200
+    b = Batch(8, 2, [(512, 512, [3, 400, 5])], seed=16)
+    b.q = b.q[:1].expand(b.B, -1, -1)
+    b.check(b.run())
+    with pytest.raises(ValueError, match="rows apart"):
+        b.run(out=torch.zeros(1, 8, 128, dtype=BF, device=DEV).expand(b.B, -1, -1))
+    one = Batch(8, 2, [], alone=[700], seed=17)
+    want = one.run()
+    odd = torch.as_strided(one.q, (1, 8, 128), (3, 128, 1))
+    into = torch.as_strided(torch.zeros_like(one.q), (1, 8, 128), (0, 128, 1))
+    assert torch.equal(one.run(q=odd, out=into), want)
+    assert b200.device_error(clear=True) == 0
+
+
+def test_two_streams_with_workspaces_of_their_own():
+    """Calls on two streams at once through the C entry, each with its own workspace."""
+    from src import b200
+    lib = b200.load_library()
+    pair = [Batch(8, 2, [(1024, 1024, [400, 3, 90] * 5)], alone=[700], seed=18),
+            Batch(16, 2, [(512, 512, [40, 1200, 8, 9])], alone=[30] * 9, seed=19)]
+    want = [b.run() for b in pair]
+    streams = [torch.cuda.Stream() for _ in pair]
+    outs, keep = [torch.zeros_like(b.q) for b in pair], []
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for b, st, out in zip(pair, streams, outs):
+            if turn == 0:
+                n = b200.shared_prefix_workspace_bytes(b.B, b.max_k, b.Hq, b.Hkv)
+                keep.append([torch.zeros(n, dtype=torch.uint8, device=DEV), i32(b.group), i32(b.prefix)])
+                torch.cuda.synchronize()
+            ws, g, p = keep[pair.index(b)]
+            rc = lib.b200_shared_prefix_attention(
+                b.q.data_ptr(), b.q.stride(0), b.B, b.kc.data_ptr(), b.vc.data_ptr(), b.kc.shape[0] * b.page,
+                b.table.data_ptr(), b.table.stride(0), b.table.shape[1], b.cu_q.data_ptr(), b.cu_k.data_ptr(), b.B,
+                b.max_k, b.Hq, b.Hkv, b.page, b.scale, g.data_ptr(), p.data_ptr(), p.numel(), out.data_ptr(),
+                out.stride(0), ws.data_ptr(), ws.numel(), st.cuda_stream)
+            assert rc == 0
+    torch.cuda.synchronize()
+    for out, w, (ws, _, _) in zip(outs, want, keep):
+        assert torch.equal(out, w)
+        assert not bool(ws[:256].any())

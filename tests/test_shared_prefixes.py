@@ -105,3 +105,13 @@ def test_pool_steps_refuse_rows_that_have_no_place(rows, counts):
     with pytest.raises(ValueError, match="step"):
         pool.step(rows, counts)
     assert pool.seq_lens.tolist() == [0] * 4
+
+
+@pytest.mark.parametrize("kw", [dict(max_num_seqs=1025), dict(block_size=128), dict(heads=(9, 1))])
+def test_a_runner_refuses_what_the_kernel_cannot(kw):
+    from types import SimpleNamespace
+    from src.engine.model_runner import ModelRunner
+    q, kv = kw.pop("heads", (16, 8))
+    config = SimpleNamespace(num_attention_heads=q, num_key_value_heads=kv)
+    with pytest.raises(ValueError, match="shared_prefix"):
+        ModelRunner(config, shared_prefix=True, device=torch.device("cpu"), **kw)
