@@ -203,7 +203,8 @@ def _rows(t: torch.Tensor) -> tuple[int, int]:
 # workspaces
 # ---------------------------------------------------------------------------
 _workspaces: dict[tuple[int, str], torch.Tensor] = {}
-_outgrown: list[torch.Tensor] = []  # kept: graphs captured with them still write there
+# kept: graphs captured with them still write there
+_outgrown: list[tuple[tuple[int, str], torch.Tensor]] = []
 
 
 def workspace(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
@@ -217,7 +218,7 @@ def workspace(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
             raise RuntimeError(f"workspace '{kind}' must be sized before CUDA-graph capture "
                                f"({nbytes} bytes requested)")
         if buf is not None:
-            _outgrown.append(buf)
+            _outgrown.append((key, buf))
         buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _workspaces[key] = buf
     return buf
@@ -253,7 +254,7 @@ def device_error(clear: bool = True) -> int:
         dev = torch.cuda.current_device()
         heads = {"attn": attention_workspace_bytes(0, 0, 1), "gemm": _GEMM_FLAG_BYTES,
                  "shared_prefix": _QUEUE_BYTES}
-        for (d, kind), buf in _workspaces.items():
+        for (d, kind), buf in [*_workspaces.items(), *_outgrown]:
             if d == dev and kind in heads:
                 buf[:heads[kind]].zero_()
         torch.cuda.synchronize()

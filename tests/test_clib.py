@@ -224,3 +224,29 @@ def test_shared_prefix_attention_refuses_cpu_tensors():
     i = torch.zeros(3, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="CUDA tensors"):
         b200.shared_prefix_attention(q, c, c, i, i, 4, 0.1, torch.zeros(2, 1, dtype=torch.int32), i[:2], i[:1])
+
+
+def test_a_timeout_clears_every_workspace_in_use(monkeypatch):
+    """After a timeout bit the heads of all workspaces are zeroed, those that
+    were outgrown (captured graphs still use them) as well."""
+    import types
+    import torch
+    from src import b200
+
+    def error_word(p, clear):
+        p._obj.value = 1
+        return 0
+    monkeypatch.setattr(b200, "load_library", lambda: types.SimpleNamespace(
+        b200_device_error=error_word, b200_attention_workspace_bytes=lambda *a: 0))
+    monkeypatch.setattr(b200, "attention_workspace_bytes", lambda *a: 512)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    bufs = {(d, k): torch.ones(8192, dtype=torch.uint8) for d in (0, 1) for k in ("attn", "gemm", "shared_prefix")}
+    old = torch.ones(1024, dtype=torch.uint8)
+    monkeypatch.setattr(b200, "_workspaces", bufs)
+    monkeypatch.setattr(b200, "_outgrown", [((0, "shared_prefix"), old)])
+    assert b200.device_error(clear=True) == 1
+    for (d, kind), buf in bufs.items():
+        head = {"attn": 512, "gemm": 4096, "shared_prefix": 256}[kind] if d == 0 else 0
+        assert int(buf.sum()) == 8192 - head
+    assert int(old.sum()) == 1024 - 256
