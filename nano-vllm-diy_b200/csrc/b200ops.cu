@@ -1692,8 +1692,10 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
   if (int r = check_launch("shared_attention_kernel")) return r;
   // the parts of each row
   const int rows = B * Hq;
-  e = launch_overlapped(rows <= ds->num_sms * 24 ? shared_merge_kernel<8> : shared_merge_kernel<4>,
-                        (rows + kMergeWarps - 1) / kMergeWarps, kMergeWarps * 32, 0, st, s);
+  const bool few = rows <= ds->num_sms * 24;
+  const int per = kMergeWarps * (few ? 1 : 2);
+  e = launch_overlapped(few ? shared_merge_kernel<8, 32> : shared_merge_kernel<4, 16>, (rows + per - 1) / per,
+                        kMergeWarps * 32, 0, st, s);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
   return check_launch("shared_merge_kernel");
 }

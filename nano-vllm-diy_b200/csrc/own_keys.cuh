@@ -461,18 +461,22 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 
 // ---------------------------------------------------------------------------
 // The parts of a row of attention with shared prefixes: the prefix's pieces,
-// then the items of the sequence's own keys, always in that order.  One warp
-// per (sequence, query head), 4 dims a lane.  The parts come from L2, so it is
-// latency that counts: kFlight parts are in flight at once, 8 where few rows
-// leave the registers for it, 4 where more resident warps are worth more.
+// then the items of the sequence's own keys, always in that order.  kLanes lanes
+// to a (sequence, query head).  The parts come from L2, so it is latency that
+// counts: kFlight parts are in flight at once.  A warp to a row and 8 parts where
+// rows are few (often of many pieces: with half a warp 4 sequences behind 16k keys
+// 33.0 us, not 30.9), half a warp and 4 parts where there are more than 24 rows an
+// SM, so that twice as many are under way (256 sequences of 32 heads: 106.9, not
+// 108.5).
 // ---------------------------------------------------------------------------
 constexpr int kMergeWarps = 4;
 
-template <int kFlight>
-__global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 9) shared_merge_kernel(const SharedArgs a) {
+template <int kFlight, int kLanes>
+__global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 7) shared_merge_kernel(const SharedArgs a) {
   griddep_wait();
   griddep_launch_dependents();
-  const int row = blockIdx.x * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  constexpr int kVecs = 32 / kLanes;  // of 4 dims a lane
+  const int row = (blockIdx.x * kMergeWarps * 32 + threadIdx.x) / kLanes, lane = threadIdx.x % kLanes;
   if (row >= a.B * a.Hq) return;
   const int b = row / a.Hq, hq = row - b * a.Hq, h = hq / a.G;
   const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0;
@@ -490,10 +494,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 9) shared
   const size_t in_block = (size_t)(rc.rank % a.members) * a.G + (hq - h * a.G);
   const int n = pieces + own;
   float M = -INFINITY, L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 acc[kVecs];
+#pragma unroll
+  for (int e = 0; e < kVecs; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < n; i0 += kFlight) {
     float2 ml[kFlight];
-    float4 o[kFlight];
+    float4 o[kFlight][kVecs];
 #pragma unroll
     for (int u = 0; u < kFlight; ++u) {
       const int i = i0 + u;
@@ -509,7 +515,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 9) shared
         po = a.part_o + at * kOwnHD;
       }
       ml[u] = i < n ? __ldcg(pm) : make_float2(-INFINITY, 0.f);
-      o[u] = i < n ? __ldcg(reinterpret_cast<const float4*>(po) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int e = 0; e < kVecs; ++e)
+        o[u][e] = i < n ? __ldcg(reinterpret_cast<const float4*>(po) + e * kLanes + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int u = 0; u < kFlight; ++u) {
@@ -517,18 +525,22 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 9) shared
       const float mn = fmaxf(M, ml[u].x);
       const float s = fast_exp2(M - mn), w = fast_exp2(ml[u].x - mn);
       L = L * s + w * ml[u].y;
-      acc.x = acc.x * s + w * o[u].x;
-      acc.y = acc.y * s + w * o[u].y;
-      acc.z = acc.z * s + w * o[u].z;
-      acc.w = acc.w * s + w * o[u].w;
+#pragma unroll
+      for (int e = 0; e < kVecs; ++e) {
+        acc[e].x = acc[e].x * s + w * o[u][e].x;
+        acc[e].y = acc[e].y * s + w * o[u][e].y;
+        acc[e].z = acc[e].z * s + w * o[u][e].z;
+        acc[e].w = acc[e].w * s + w * o[u][e].w;
+      }
       M = mn;
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  uint2 packed;
-  packed.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-  packed.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(a.out + (size_t)q0 * a.out_stride + (size_t)hq * kOwnHD + lane * 4) = packed;
+  uint2* out = reinterpret_cast<uint2*>(a.out + (size_t)q0 * a.out_stride + (size_t)hq * kOwnHD);
+#pragma unroll
+  for (int e = 0; e < kVecs; ++e)
+    out[e * kLanes + lane] =
+        make_uint2(pack_bf16x2(acc[e].x * inv, acc[e].y * inv), pack_bf16x2(acc[e].z * inv, acc[e].w * inv));
 }
 
 }  // namespace b200
