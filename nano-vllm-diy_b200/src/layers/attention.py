@@ -31,9 +31,11 @@ def attend(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
            k_cache: torch.Tensor, v_cache: torch.Tensor, ctx: Context, scale: float,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over the batch described by ctx (no cache write)."""
-    if ctx.prefix_group is not None and ctx.block_tables is not None and ctx.max_seqlen_q == 1:
+    # (a tree with its own Context, to which these layers are copied, has no such fields)
+    group = getattr(ctx, "prefix_group", None)
+    if group is not None and ctx.block_tables is not None and ctx.max_seqlen_q == 1:
         return b200.shared_prefix_attention(q, k_cache, v_cache, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
-                                            ctx.max_seqlen_k, scale, ctx.block_tables, ctx.prefix_group,
+                                            ctx.max_seqlen_k, scale, ctx.block_tables, group,
                                             ctx.prefix_lens, out=out)
     if ctx.block_tables is not None:
         return b200.paged_attention(q, None, None, k_cache, v_cache, ctx.cu_seqlens_q,
