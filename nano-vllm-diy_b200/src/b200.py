@@ -9,12 +9,14 @@ device, the call fails.
 The decode-attention workspace (its scheduler counters and split-KV partials)
 and the GEMM workspace (split-K flags and fp32 partials of the SM-pair GEMM)
 are per-device torch buffers that grow on demand outside CUDA-graph capture
-and are reused by every call.
+and are reused by every call; the shared-prefix workspace is one per stream,
+or the caller's.
 """
 from __future__ import annotations
 
 import ctypes
 import os
+import weakref
 
 import torch
 
@@ -145,6 +147,7 @@ def _bf16(*ts: torch.Tensor | None) -> None:
 
 # the current stream's handle without the Stream object around it (several us a call)
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_stream_captured = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _device_of(*ts: torch.Tensor | None) -> int:
@@ -224,9 +227,15 @@ def workspace(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
     return buf
 
 
-def reserve_workspace(kind: str, nbytes: int, device: torch.device) -> None:
-    workspace(kind, nbytes, device)
+def _stream_kind(kind: str, stream: int) -> str:
+    """Key of a workspace that every stream has one of its own of."""
+    return kind if stream == 0 else f"{kind}@{stream:x}"
 
+
+def reserve_workspace(kind: str, nbytes: int, device: torch.device) -> None:
+    if kind == "shared_prefix":
+        kind = _stream_kind(kind, torch.cuda.current_stream(device).cuda_stream)
+    workspace(kind, nbytes, device)
 
 
 
@@ -255,8 +264,13 @@ def device_error(clear: bool = True) -> int:
         heads = {"attn": attention_workspace_bytes(0, 0, 1), "gemm": _GEMM_FLAG_BYTES,
                  "shared_prefix": _QUEUE_BYTES}
         for (d, kind), buf in [*_workspaces.items(), *_outgrown]:
+            kind = kind.partition("@")[0]
             if d == dev and kind in heads:
                 buf[:heads[kind]].zero_()
+        for ref in _prefix_workspaces:
+            buf = ref()
+            if buf is not None and buf.get_device() == dev:
+                buf[:_QUEUE_BYTES].zero_()
         torch.cuda.synchronize()
     return v.value
 
@@ -632,7 +646,33 @@ def shared_prefix_workspace_bytes(max_seqs: int, max_seqlen_k: int, num_heads: i
     return int(size.value)
 
 
-def _prefix_workspace(dev: int, *shape: int) -> torch.Tensor:
+# the ones that callers hold: device_error() zeroes their heads after a timeout
+_prefix_workspaces: list[weakref.ref] = []
+
+
+def shared_prefix_workspace(max_seqs: int, max_seqlen_k: int, num_heads: int, num_kv_heads: int,
+                            device: torch.device | None = None) -> torch.Tensor:
+    """A workspace for the calls of shared_prefix_attention that are given it, up to these sizes."""
+    device = device or torch.device("cuda", torch.cuda.current_device())
+    with torch.cuda.device(device):
+        n = shared_prefix_workspace_bytes(max_seqs, max_seqlen_k, num_heads, num_kv_heads)
+    buf = torch.zeros(n, dtype=torch.uint8, device=device)
+    _prefix_workspaces[:] = [r for r in _prefix_workspaces if r() is not None]
+    _prefix_workspaces.append(weakref.ref(buf))
+    return buf
+
+
+def _capturing(dev: int) -> bool:
+    if dev == torch._C._cuda_getDevice():
+        return _stream_captured()
+    with torch.cuda.device(dev):
+        return _stream_captured()
+
+
+def _prefix_workspace(dev: int, given: torch.Tensor | None, *shape: int) -> torch.Tensor:
+    """The workspace of one call.  Two launches use it, one after the other, and calls that share it
+    must not overlap on the GPU: so each stream has one, and a captured call one in its graph's
+    memory, its head zeroed by the graph itself (graphs may be replayed on any streams)."""
     key = (dev, *shape)
     n = _prefix_ws_bytes.get(key)
     if n is None:
@@ -641,21 +681,39 @@ def _prefix_workspace(dev: int, *shape: int) -> torch.Tensor:
         if len(_prefix_ws_bytes) >= 4096:
             _prefix_ws_bytes.clear()
         _prefix_ws_bytes[key] = n
-    buf = _workspaces.get((dev, "shared_prefix"))
-    return buf if buf is not None and buf.numel() >= n else workspace("shared_prefix", n, torch.device("cuda", dev))
+    if given is not None:
+        if given.dtype is not torch.uint8 or given.dim() != 1 or not given.is_contiguous():
+            raise TypeError("workspace must be a contiguous uint8 vector")
+        if given.numel() < n or given.data_ptr() % 256:
+            raise ValueError(f"workspace of {given.numel()} bytes: {n} needed, on a 256-byte boundary")
+        return given
+    stream = _raw_stream(dev)
+    if stream != 0 and _capturing(dev):  # (the default stream cannot be captured)
+        buf = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", dev))
+        buf[:_QUEUE_BYTES].zero_()
+        return buf
+    kind = _stream_kind("shared_prefix", stream)
+    buf = _workspaces.get((dev, kind))
+    return buf if buf is not None and buf.numel() >= n else workspace(kind, n, torch.device("cuda", dev))
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                             cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, max_seqlen_k: int,
                             softmax_scale: float, block_table: torch.Tensor, prefix_group: torch.Tensor,
-                            prefix_len: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+                            prefix_len: torch.Tensor, out: torch.Tensor | None = None,
+                            workspace: torch.Tensor | None = None) -> torch.Tensor:
     """paged_attention of a decode batch (one query per sequence) whose sequences share prefixes.
 
     prefix_group int32 [B]: the group of each sequence, -1 for none; prefix_len int32 [groups]: the
     keys shared in each group, that is, the first prefix_len // page pages of the block tables of its
     sequences are the same (src.engine.metadata.shared_prefixes finds such groups).  The keys of a
-    prefix are read once for its whole group."""
-    dev = _device_of(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, prefix_group, prefix_len, out)
+    prefix are read once for its whole group.
+
+    workspace: from shared_prefix_workspace(), for calls that never overlap on the GPU.  Without it,
+    eager calls use one of their stream, and a captured call one of its graph, which zeroes 256 bytes
+    of it in front of the call."""
+    dev = _device_of(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, prefix_group, prefix_len, out,
+                     workspace)
     _bf16(q, k_cache, v_cache, out)
     B = _index("cu_seqlens_q", cu_seqlens_q) - 1
     _index("cu_seqlens_k", cu_seqlens_k, B + 1)
@@ -683,7 +741,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise ValueError(f"out must be {tuple(q.shape)} with contiguous heads and rows apart")
     pages, page, Hkv, _ = cache
     max_k = int(max_seqlen_k)
-    ws = _prefix_workspace(dev, B, max_k, Hq, Hkv)
+    ws = _prefix_workspace(dev, workspace, B, max_k, Hq, Hkv)
     _call("b200_shared_prefix_attention", dev, q.data_ptr(), q_stride[0] if T > 1 else row, T, k_cache.data_ptr(), v_cache.data_ptr(),
           pages * page, block_table.data_ptr(), stride[0], table[1], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
           B, max_k, Hq, Hkv, page, softmax_scale, prefix_group.data_ptr(), prefix_len.data_ptr(), groups,

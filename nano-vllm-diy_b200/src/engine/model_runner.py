@@ -209,6 +209,9 @@ class ModelRunner:
             # groups of two at least; a sequence in none has -1
             v["prefix_group"] = torch.full((max_bs,), -1, dtype=torch.int32, device=dev)
             v["prefix_lens"] = torch.zeros(max(max_bs // 2, 1), dtype=torch.int32, device=dev)
+            # of this runner's graphs, which run one after the other
+            v["prefix_workspace"] = b200.shared_prefix_workspace(max_bs, self.max_seq_len, self.local_q_heads,
+                                                                 self.local_kv_heads, dev)
         self.graph_with_sampling = with_sampling
         self.graph_vars = v
         for bs in sorted(batch_sizes, reverse=True):
@@ -219,6 +222,7 @@ class ModelRunner:
             if self.shared_prefix:
                 ctx.prefix_group = v["prefix_group"][:bs]
                 ctx.prefix_lens = v["prefix_lens"][:max(bs // 2, 1)]
+                ctx.prefix_workspace = v["prefix_workspace"]
             def step():
                 v["outputs"][:bs] = self.model(v["input_ids"][:bs], v["positions"][:bs], ctx)
                 if with_sampling:

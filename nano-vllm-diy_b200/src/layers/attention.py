@@ -36,7 +36,8 @@ def attend(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
     if group is not None and ctx.block_tables is not None and ctx.max_seqlen_q == 1:
         return b200.shared_prefix_attention(q, k_cache, v_cache, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
                                             ctx.max_seqlen_k, scale, ctx.block_tables, group,
-                                            ctx.prefix_lens, out=out)
+                                            ctx.prefix_lens, out=out,
+                                            workspace=getattr(ctx, "prefix_workspace", None))
     if ctx.block_tables is not None:
         return b200.paged_attention(q, None, None, k_cache, v_cache, ctx.cu_seqlens_q,
                                     ctx.cu_seqlens_k, ctx.max_seqlen_q, ctx.max_seqlen_k, scale,

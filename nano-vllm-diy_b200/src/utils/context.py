@@ -1,7 +1,8 @@
 """Per-step attention metadata, the same record as the reference's
 src/utils/context.py:5-14 (field names, order and defaults are part of the
 interface that ModelRunner fills in and the layers read), and behind its
-fields the groups of sequences that share a prefix, for decode batches."""
+fields the groups of sequences that share a prefix, for decode batches, and
+the workspace of the attention over them."""
 from dataclasses import dataclass
 
 from torch import Tensor
@@ -19,3 +20,4 @@ class Context:
     block_tables: Tensor | None = None      # int32 [B, max_blocks], -1 padded
     prefix_group: Tensor | None = None      # int32 [B], group of each sequence or -1
     prefix_lens: Tensor | None = None       # int32 [groups], keys shared in each group
+    prefix_workspace: Tensor | None = None  # of b200.shared_prefix_workspace; None: the stream's or the graph's
