@@ -121,6 +121,14 @@ int device_state(DeviceState** out) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
   if (dev < 0 || dev >= kMaxDevices) return fail(B200_ERR_INVALID, "device %d out of range", dev);
+  // A host thread that has not used the device yet has no context, which the
+  // driver's tensor map encoder needs; naming the device makes it current.
+  thread_local int current = -1;
+  if (current != dev) {
+    e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return fail(B200_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(e));
+    current = dev;
+  }
   DeviceState& s = g_dev[dev];
   if (!s.init) {
     e = cudaDeviceGetAttribute(&s.num_sms, cudaDevAttrMultiProcessorCount, dev);
