@@ -41,6 +41,14 @@ thread_local std::string g_last_error;
 // leaf functions, which never call one another while holding it.
 std::mutex g_host_mutex;
 
+// Held while a call makes its launches, by the calls of several launches that
+// leave something for one another (parts of rows in a workspace, a plan for
+// the tables) and those that change the same tables: the launches of calls
+// that host threads make on one stream must not come in between.  By stream,
+// since a launch can wait for room in its stream's queue.
+std::mutex g_stream_order[64];
+std::mutex& stream_order(cudaStream_t st) { return g_stream_order[(reinterpret_cast<uintptr_t>(st) >> 4) % 64]; }
+
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -1694,6 +1702,7 @@ extern "C" int b200_shared_prefix_attention(const void* q, long long q_stride, i
     return r;
   if (int r = check_shared_registers()) return r;
   if (int r = ensure_smem(ds, 32u, shared_attention_kernel, kSharedSmemBytes)) return r;
+  std::lock_guard<std::mutex> order(stream_order(st));
   cudaError_t e = launch_ex(shared_attention_kernel, dim3(ds->num_sms), dim3(kSpThreads), kSharedSmemBytes, st,
                             nullptr, 0, tmK, tmV, tmQ, s);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "shared_prefix launch: %s", cudaGetErrorString(e));
@@ -1763,8 +1772,10 @@ extern "C" int b200_copy_pages(void* cache, long long s0, long long s1, long lon
   DeviceState* ds;
   if (int r = device_state(&ds)) return r;
   const long long units = (long long)n * c.planes * ((c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs);
-  launch_ex(copy_pages_kernel, dim3((unsigned)std::min<long long>(units, kPgGrid)), dim3(kPgThreads), 0, reinterpret_cast<cudaStream_t>(stream),
-            nullptr, 0, c, src, dst, num_tokens, n, num_pages, page, ds->err);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  std::lock_guard<std::mutex> order(stream_order(st));
+  launch_ex(copy_pages_kernel, dim3((unsigned)std::min<long long>(units, kPgGrid)), dim3(kPgThreads), 0, st, nullptr, 0,
+            c, src, dst, num_tokens, n, num_pages, page, ds->err);
   return check_launch("copy_pages_kernel");
 }
 
@@ -1777,8 +1788,9 @@ extern "C" int b200_take_pages(int* block_tables, long long bt_stride, int rows,
   PageTables t{};
   if (int r = page_tables("take_pages", block_tables, bt_stride, rows, width, seq_lens, refs, num_pages, page, &t))
     return r;
-  launch_ex(take_pages_kernel, dim3(1), dim3(kPgMax), 0, reinterpret_cast<cudaStream_t>(stream), nullptr, 0, t,
-            row_ids, new_lens, n, done);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  std::lock_guard<std::mutex> order(stream_order(st));
+  launch_ex(take_pages_kernel, dim3(1), dim3(kPgMax), 0, st, nullptr, 0, t, row_ids, new_lens, n, done);
   return check_launch("take_pages_kernel");
 }
 
@@ -1789,8 +1801,9 @@ extern "C" int b200_free_pages(int* block_tables, long long bt_stride, int rows,
   PageTables t{};
   if (int r = page_tables("free_pages", block_tables, bt_stride, rows, width, seq_lens, refs, num_pages, 1, &t))
     return r;
-  launch_ex(free_pages_kernel, dim3(n), dim3(kPgThreads), 0, reinterpret_cast<cudaStream_t>(stream), nullptr, 0, t,
-            row_ids);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  std::lock_guard<std::mutex> order(stream_order(st));
+  launch_ex(free_pages_kernel, dim3(n), dim3(kPgThreads), 0, st, nullptr, 0, t, row_ids);
   return check_launch("free_pages_kernel");
 }
 
@@ -1808,6 +1821,7 @@ extern "C" int b200_fork_pages(void* cache, long long s0, long long s1, long lon
   if (int r = page_tables("fork_pages", block_tables, bt_stride, rows, width, seq_lens, refs, num_pages, page, &t))
     return r;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  std::lock_guard<std::mutex> order(stream_order(st));
   launch_ex(fork_plan_kernel, dim3(1), dim3(kPgMax), 0, st, nullptr, 0, t, parents, children, n, plan, done);
   if (int r = check_launch("fork_plan_kernel")) return r;
   const long long units = n + (long long)n * c.planes * ((c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs);
@@ -1828,6 +1842,7 @@ extern "C" int b200_compact_pages(void* cache, long long s0, long long s1, long 
   if (int r = page_tables("compact_pages", block_tables, bt_stride, rows, width, nullptr, refs, num_pages, page, &t))
     return r;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  std::lock_guard<std::mutex> order(stream_order(st));
   launch_ex(compact_plan_kernel, dim3(1), dim3(kPgMax), 0, st, nullptr, 0, t, place, moves);
   if (int r = check_launch("compact_plan_kernel")) return r;
   const long long pieces = (c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs;

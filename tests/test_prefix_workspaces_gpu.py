@@ -95,3 +95,94 @@ def test_workspace_of_the_caller():
     assert not bool(ws[:256].any())
     with pytest.raises(ValueError, match="needed"):
         made[0].run(workspace=ws[:4096], **made[0].args)
+
+
+def in_threads(*loops):
+    """The loops at once, each on a host thread of its own; the first exception is raised here."""
+    import sys
+    import threading
+    failed, gate = [], threading.Barrier(len(loops))
+
+    def body(loop):
+        try:
+            gate.wait(60)
+            loop()
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-5)
+    threads = [threading.Thread(target=body, args=(loop,)) for loop in loops]
+    try:
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(interval)
+    torch.cuda.synchronize()
+    if failed:
+        raise failed[0]
+
+
+def test_host_threads_on_one_stream():
+    """The launches of a call stay together: with one workspace and one stream,
+    calls of two threads would otherwise merge each other's parts."""
+    made = batches()
+    outs = [[torch.zeros_like(b.q) for _ in range(150)] for b in made]
+    torch.cuda.synchronize()
+    in_threads(*[lambda b=b, out=out: [b.run(out=o, **b.args) for o in out] for b, out in zip(made, outs)])
+    for b, out in zip(made, outs):
+        for o in out:
+            assert torch.equal(o, b.want)
+
+
+def test_host_threads_on_the_tables_of_one_pool():
+    """Forks, turnovers and compactions of three threads on one stream: in
+    whatever order the calls come, the tables hold together and every row has
+    its tokens."""
+    from src.engine.pages import PagePool
+    pages, page = 160, 16
+    kv = torch.zeros(2, 2, pages, page, 1, 8, dtype=torch.bfloat16, device=DEV)
+    pool = PagePool(kv, 16, 8 * page)
+    lens = [100, 37, 64, 5, 128, 81]
+    assert pool.take(list(range(6)), lens).tolist() == [1] * 6
+
+    def slots(row, n):
+        table = pool.block_tables[row].tolist()
+        return [table[i // page] * page + i % page for i in range(n)]
+
+    flat = kv.view(2, 2, pages * page, 8)
+    for r, n in enumerate(lens):
+        flat[:, :, slots(r, n)] = (torch.arange(n, device=DEV) % 16 + 16 * r).to(kv.dtype)[None, None, :, None]
+    rows = {r: i32([r]) for r in range(16)}
+    most = i32([7 * page])
+    torch.cuda.synchronize()
+
+    def forks():
+        for i in range(150):
+            pool.free(rows[10])
+            pool.fork(rows[i % 6], rows[10])
+
+    def turnovers():
+        for _ in range(150):
+            pool.free(rows[11])
+            pool.take(rows[11], most)
+
+    def compactions():
+        for _ in range(150):
+            pool.compact()
+
+    in_threads(forks, turnovers, compactions)
+    table = pool.block_tables.tolist()
+    held = [0] * pages
+    for r, entries in enumerate(table):
+        n = -(-pool.seq_lens[r].item() // page)
+        assert min(entries[:n], default=0) >= 0 and set(entries[n:]) <= {-1}, r
+        for e in entries[:n]:
+            held[e] += 1
+    assert pool.refs.tolist() == held
+    assert pool.seq_lens.tolist() == lens + [0] * 4 + [lens[149 % 6], 7 * page] + [0] * 4
+    for r, of in [*((r, r) for r in range(6)), (10, 149 % 6)]:
+        want = (torch.arange(lens[of], device=DEV) % 16 + 16 * of).to(kv.dtype)
+        assert torch.equal(flat[:, :, slots(r, lens[of])], want[None, None, :, None].expand(2, 2, -1, 8)), r
