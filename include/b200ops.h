@@ -311,7 +311,8 @@ int b200_shared_prefix_workspace_bytes(int max_seqs, int max_seqlen_k, int Hq, i
  *    softmax_scale > 0.
  *  - Sequences longer than max_seqlen_k may not fit the workspace's places for
  *    parts of a row; then B200_DEVERR_BAD_INDEX is set and the output is not
- *    to be used.  It is also set for a query row outside q (left out) and for
+ *    to be used.  It is also set for a sequence of more than one query or with
+ *    a query row outside q (left out: its rows of out stay as they were) and for
  *    missing pages (their keys count for nothing).
  *  - workspace: b200_shared_prefix_workspace_bytes(B, max_seqlen_k, Hq, Hkv) bytes,
  *    256-byte aligned, its first 256 bytes zero before the first call (they

@@ -128,8 +128,8 @@ __device__ __forceinline__ void own_run(const SharedArgs& a, uint8_t* smem, cons
       const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0;
       const int nk = a.cu_k[b + 1] - a.cu_k[b] - p;
       s.prefix[b] = p;
-      // own keys, for now (a row outside q has no place to go: sp_group_of reports it)
-      s.start[b] = nq >= 1 && q0 >= 0 && q0 < a.num_q_rows ? max(nk, 0) : 0;
+      // own keys, for now (a row outside q, or of several queries, has no place to go: sp_group_of reports it)
+      s.start[b] = nq == 1 && q0 >= 0 && q0 < a.num_q_rows ? max(nk, 0) : 0;
       keys += s.start[b];
       active += s.start[b] > 0;
     }
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kFlight == 8 ? 6 : 7) shared
   const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0;
   const int c0 = a.starts[b], own = a.starts[b + 1] - c0;
   const SpRec rc = a.rec[b];
-  if (nq < 1 || (own == 1 && rc.keys == 0)) return;  // padding; written by its one item
+  if (nq != 1 || (own == 1 && rc.keys == 0)) return;  // padding, or reported with the plan; written by its one item
   if (q0 < 0 || q0 >= a.num_q_rows) return;            // reported with the plan
   if (c0 < 0 || own < 0 || (long long)c0 + own > a.cap_items) {  // lengths past max_seqlen_k: no such parts
     if (lane == 0) raise_error(a.err, ERR_BAD_INDEX);

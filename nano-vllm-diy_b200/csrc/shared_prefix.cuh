@@ -222,7 +222,7 @@ __device__ __forceinline__ int sp_div(int a, int b) {
 __device__ __forceinline__ int sp_group_of(const SharedArgs& a, int b, bool flag = false) {
   const int g = a.prefix_group[b];
   const int q0 = a.cu_q[b], nq = a.cu_q[b + 1] - q0, nk = a.cu_k[b + 1] - a.cu_k[b];
-  if (g < -1 || g >= a.groups || (nq >= 1 && (q0 < 0 || q0 >= a.num_q_rows))) {
+  if (g < -1 || g >= a.groups || nq > 1 || (nq == 1 && (q0 < 0 || q0 >= a.num_q_rows))) {
     if (flag) raise_error(a.err, ERR_BAD_INDEX);
     return -1;
   }
@@ -238,7 +238,7 @@ __device__ __forceinline__ void sp_count_groups(const SharedArgs& a, int* cnt, i
   auto row = [&](int b, int& nk) {
     nk = 0;
     if (b >= a.B) return -1;
-    nk = a.cu_q[b + 1] > a.cu_q[b] ? max(a.cu_k[b + 1] - a.cu_k[b], 0) : 0;
+    nk = a.cu_q[b + 1] - a.cu_q[b] == 1 ? max(a.cu_k[b + 1] - a.cu_k[b], 0) : 0;
     return sp_group_of(a, b, blockIdx.x == 0);
   };
   int nk, g = row(tid, nk);  // (the loads of the first rows are on their way during the barrier)

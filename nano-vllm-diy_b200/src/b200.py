@@ -707,7 +707,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     prefix_group int32 [B]: the group of each sequence, -1 for none; prefix_len int32 [groups]: the
     keys shared in each group, that is, the first prefix_len // page pages of the block tables of its
     sequences are the same (src.engine.metadata.shared_prefixes finds such groups).  The keys of a
-    prefix are read once for its whole group.
+    prefix are read once for its whole group.  A sequence of more than one query is left out (its
+    rows of out stay as they were) and flagged as a bad index (device_error).
 
     workspace: from shared_prefix_workspace(), for calls that never overlap on the GPU.  Without it,
     eager calls use one of their stream, and a captured call one of its graph, which zeroes 256 bytes
