@@ -140,6 +140,9 @@ class ModelRunner:
         if ctx.max_seqlen_q != 1 or self.enforce_eager or not self.graphs or bs > max(self.graphs):
             return self.model(input_ids, positions, ctx), ctx
         gbs = next(x for x in sorted(self.graphs) if x >= bs)
+        if self.shared_prefix and ctx.prefix_group is not None and ctx.prefix_lens.size(0) > max(gbs // 2, 1):
+            # more groups than the graph has places for: a caller's, some of one sequence or none
+            return self.model(input_ids, positions, ctx), ctx
         v = self.graph_vars
         v["input_ids"][:bs] = input_ids
         v["positions"][:bs] = positions
