@@ -206,24 +206,32 @@ def _rows(t: torch.Tensor) -> tuple[int, int]:
 # workspaces
 # ---------------------------------------------------------------------------
 _workspaces: dict[tuple[int, str], torch.Tensor] = {}
-# kept: graphs captured with them still write there
+# those that a capture has used; an outgrown one of them is kept, its graph still writes there
+_captured: set[tuple[int, str]] = set()
 _outgrown: list[tuple[tuple[int, str], torch.Tensor]] = []
 
 
 def workspace(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
     """Zero-filled on (re)allocation: both workspaces start with counters or
     flags that must be zero before the first call (every call leaves them
-    zero)."""
+    zero).  It grows to what is asked for, or at least twofold where the old
+    one has to be kept for a graph, so that the kept ones are never more than
+    the one in use."""
     key = (device.index if device.index is not None else torch.cuda.current_device(), kind)
     buf = _workspaces.get(key)
+    capturing = _raw_stream(key[0]) != 0 and _stream_captured()  # (the default stream cannot be captured)
     if buf is None or buf.numel() < nbytes:
-        if torch.cuda.is_current_stream_capturing():
+        if capturing:
             raise RuntimeError(f"workspace '{kind}' must be sized before CUDA-graph capture "
                                f"({nbytes} bytes requested)")
-        if buf is not None:
+        if key in _captured:
+            _captured.discard(key)
             _outgrown.append((key, buf))
+            nbytes = max(nbytes, 2 * buf.numel())
         buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _workspaces[key] = buf
+    elif capturing:
+        _captured.add(key)
     return buf
 
 
