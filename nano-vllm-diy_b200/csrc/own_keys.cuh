@@ -239,7 +239,7 @@ __device__ __forceinline__ void own_run(const SharedArgs& a, uint8_t* smem, cons
           off = 0;
           ++col;
         }
-        ok = stage_free();
+        ok = __all_sync(0xffffffffu, stage_free());  // (each lane has a clock of its own: they leave together)
         if (!ok) break;
         if (lane == 0) {
           if (!there) raise_error(a.err, ERR_BAD_INDEX);

@@ -564,7 +564,10 @@ __device__ __forceinline__ void sp_run_jobs(const SharedArgs& a, const SpSmem& s
       const bool leader = sp_elect();
       int it = 0, seg[2] = {0, 0}, step[2] = {0, 0};
       bool ok = true;
-      auto wait_slot = [&](int i) { return mbar_wait(&full[i % kSpSlots], (uint32_t)(i / kSpSlots) & 1u, a.err); };
+      // (each lane has a clock of its own: they give up together)
+      auto wait_slot = [&](int i) {
+        return __all_sync(0xffffffffu, mbar_wait(&full[i % kSpSlots], (uint32_t)(i / kSpSlots) & 1u, a.err)) != 0;
+      };
       auto scores = [&](int t, int i) {  // S_t = Q_t K^T, K in load i
         const uint64_t q = dq + (uint32_t)t * 2048u, k = dk + (uint32_t)(i % kSpSlots) * 2048u;
         if (leader) {
@@ -598,7 +601,7 @@ __device__ __forceinline__ void sp_run_jobs(const SharedArgs& a, const SpSmem& s
           tc_fence_after();
           if (ok) scores(t, it);
         }
-        if (!__all_sync(0xffffffffu, ok)) break;
+        if (!ok) break;
         commit(&empty[it % kSpSlots]);
         for (int k = g.k0; k < g.k1; ++k, it += 2) {
           const bool more = k + 1 < g.k1;
@@ -618,7 +621,6 @@ __device__ __forceinline__ void sp_run_jobs(const SharedArgs& a, const SpSmem& s
             // S_t's next scores overwrite P_t: MMAs of one thread run in the order of issue
             if (more && t == 0) {
               ok = wait_slot(it + 2);
-              ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
             }
             if (more) scores(t, it + 2);
