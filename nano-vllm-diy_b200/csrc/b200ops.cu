@@ -1846,7 +1846,8 @@ extern "C" int b200_compact_pages(void* cache, long long s0, long long s1, long 
   launch_ex(compact_plan_kernel, dim3(1), dim3(kPgMax), 0, st, nullptr, 0, t, place, moves);
   if (int r = check_launch("compact_plan_kernel")) return r;
   const long long pieces = (c.page_vecs + kPgPieceVecs - 1) / kPgPieceVecs;
-  const long long units = ((long long)rows * width + kPgThreads - 1) / kPgThreads + num_pages / 2 * c.planes * pieces;
+  const long long units =
+      ((long long)rows * width + kPgThreads - 1) / kPgThreads + (long long)(num_pages / 2) * c.planes * pieces;
   launch_overlapped(compact_apply_kernel, (int)std::min<long long>(units, kPgGridUnknown), kPgThreads, 0, st, t, c,
                     static_cast<const int*>(place), static_cast<const int*>(moves));
   return check_launch("compact_apply_kernel");
