@@ -55,6 +55,7 @@ constexpr int kSpThreads = 384;
 constexpr int kSpRegsLaunch = 168, kSpRegsIssue = 88, kSpRegsSoftmax = 208;
 static_assert(kSpRegsIssue + 2 * kSpRegsSoftmax == 3 * kSpRegsLaunch, "the shares are what the launch has");
 constexpr float kSpLazy = 8.f;
+constexpr float kSpFused = 4096.f;  // maxima (log2) beyond which scores are scaled before the difference
 constexpr int kSpQ = 0;                            // [2 tiles][2 dim halves][128 rows][128 B]
 constexpr int kSpRing = 65536;
 constexpr int kSpPlanAt = kSpRing + kSpSlots * 32768;
@@ -726,7 +727,17 @@ __device__ __forceinline__ void sp_run_jobs(const SharedArgs& a, const SpSmem& s
           m = m_new;
         }
         const float mm = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: P = 0
-        const F2 scale2 = {a.scale_log2, a.scale_log2}, minus = {-mm, -mm};
+        F2 scale2 = {a.scale_log2, a.scale_log2};
+        const F2 minus = {-mm, -mm};
+        // The fused s scale - mm keeps what was rounded off in mm, up to 2^-24 of it:
+        // nothing beside the rounding of P as long as mm is small, but at the
+        // lowest value of a type (masked keys) 2^100 and more.  There the product is
+        // rounded first, as the maximum and the own keys' scores are.
+        if (__any_sync(0xffffffffu, fabsf(mm) > kSpFused)) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) s[i] *= a.scale_log2;
+          scale2 = {1.f, 1.f};
+        }
         F2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
