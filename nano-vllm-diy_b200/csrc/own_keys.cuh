@@ -333,7 +333,8 @@ __device__ __forceinline__ void own_run(const SharedArgs& a, uint8_t* smem, cons
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int tok = 16 * mt + g + 8 * (i >> 1);
-          x[mt][i] = tok < d.ntok ? (sc[mt][0][i] + sc[mt][1][i]) * a.scale_log2 : -INFINITY;
+          // (never fused with the difference below: see kSpFused)
+          x[mt][i] = tok < d.ntok ? __fmul_rn(sc[mt][0][i] + sc[mt][1][i], a.scale_log2) : -INFINITY;
           cm[i & 1] = fmaxf(cm[i & 1], x[mt][i]);
         }
       }
