@@ -123,20 +123,44 @@ DeviceState g_dev[kMaxDevices];
 
 __device__ unsigned g_device_error_word;
 
+PFN_cuCtxGetCurrent_v4000 current_context_fn() {
+  static PFN_cuCtxGetCurrent_v4000 fn = nullptr;
+  std::lock_guard<std::mutex> lock(g_host_mutex);
+  if (fn == nullptr) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuCtxGetCurrent", &p, 4000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuCtxGetCurrent_v4000>(p);
+  }
+  return fn;
+}
+
+// A host thread that has not used the GPU yet has no context, which the
+// driver's tensor map encoder needs: naming the device makes its primary one
+// current.  A context that the caller made current stays.
+int ensure_context() {
+  thread_local bool there = false;
+  if (there) return B200_OK;
+  const PFN_cuCtxGetCurrent_v4000 get = current_context_fn();
+  CUcontext ctx = nullptr;
+  if (get == nullptr || get(&ctx) != CUDA_SUCCESS || ctx == nullptr) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return fail(B200_ERR_CUDA, "no CUDA context: %s", cudaGetErrorString(e));
+  }
+  there = true;
+  return B200_OK;
+}
+
 int device_state(DeviceState** out) {
+  if (int r = ensure_context()) return r;
   std::lock_guard<std::mutex> lock(g_host_mutex);
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
   if (dev < 0 || dev >= kMaxDevices) return fail(B200_ERR_INVALID, "device %d out of range", dev);
-  // A host thread that has not used the device yet has no context, which the
-  // driver's tensor map encoder needs; naming the device makes it current.
-  thread_local int current = -1;
-  if (current != dev) {
-    e = cudaSetDevice(dev);
-    if (e != cudaSuccess) return fail(B200_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(e));
-    current = dev;
-  }
   DeviceState& s = g_dev[dev];
   if (!s.init) {
     e = cudaDeviceGetAttribute(&s.num_sms, cudaDevAttrMultiProcessorCount, dev);
