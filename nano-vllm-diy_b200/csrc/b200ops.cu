@@ -9,6 +9,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -62,7 +63,7 @@ int fail(int code, const char* fmt, ...) {
 
 // Number of kernels this library has launched from the host (graph replays
 // launch without the host and are not counted).
-unsigned long long g_launches = 0;
+std::atomic<unsigned long long> g_launches{0};
 
 int check_launch(const char* what) {
   ++g_launches;

@@ -45,3 +45,25 @@ def test_a_matrix_product_is_the_first_call_of_a_thread():
     out = torch.zeros(16, 256, dtype=torch.bfloat16, device="cuda")
     want = b200.linear(x, w)
     assert torch.equal(in_fresh_thread(lambda: b200.linear(x, w, out=out)), want)
+
+
+def test_launches_of_several_threads_are_all_counted():
+    from src import b200
+    x = torch.randn(4, 256, device="cuda").to(torch.bfloat16)
+    outs = [torch.empty(4, dtype=torch.int64, device="cuda") for _ in range(4)]
+    b200.argmax(x)
+    torch.cuda.synchronize()
+    before = b200.launch_count()
+    lib, stream = b200.load_library(), torch.cuda.current_stream().cuda_stream
+
+    def many(out):
+        for _ in range(500):
+            assert lib.b200_argmax(x.data_ptr(), x.stride(0), 4, 256, out.data_ptr(), stream) == 0
+    threads = [threading.Thread(target=many, args=(o,)) for o in outs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert b200.launch_count() - before == 2000
+    assert all(torch.equal(o, x.float().argmax(-1)) for o in outs)
