@@ -9,8 +9,9 @@
  *   - Strides are in ELEMENTS between consecutive rows (tokens).
  *   - Calls launch on `stream` and return immediately; nothing is allocated
  *     and nothing synchronises, so every call can be captured in a CUDA graph.
- *   - Host threads may call at once.  The launches of a shared-prefix or page
- *     operator stay together on its stream; the order of the calls is theirs.
+ *   - Host threads may call at once.  What a shared-prefix or page operator
+ *     launches stays together on its stream then; the order of the calls is
+ *     the threads'.  A workspace belongs to one stream at a time.
  *   - Return value: B200_OK (0) or a negative status; b200_last_error()
  *     returns the message of the calling thread's last failure.
  *   - Kernels never trap.  Out-of-range slot / block-table entries and
