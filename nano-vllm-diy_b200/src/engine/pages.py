@@ -55,7 +55,8 @@ class PagePool:
         b200.free_pages(self.block_tables, self.seq_lens, self.refs, self._vec(rows))
 
     def compact(self) -> torch.Tensor:
-        """Live pages into the front of the cache; returns where each page went (-1: free)."""
+        """Live pages into the front of the cache; returns where each page went (-1: free).  The contexts of
+        steps prepared before it name the old places."""
         return b200.compact_pages(self.kv_cache, self.block_tables, self.refs)
 
     def copy(self, src, dst, num_tokens=None) -> None:
